@@ -73,6 +73,35 @@ class TaskEx(ctypes.Structure):
                 ("rms_norm", ctypes.c_int), ("norm_eps", ctypes.c_float), ("norm_weight", ctypes.c_void_p)]
 
 
+class LoraTask(ctypes.Structure):
+    """struct q4k_lora_task (include/q4k_gemv.h): the adapters of one projection."""
+    _fields_ = [("x", ctypes.c_void_p), ("base", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("A", ctypes.c_void_p),
+                ("B", ctypes.c_void_p), ("ranks", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("K", ctypes.c_int64), ("nrows", ctypes.c_int64), ("stride_col_x", ctypes.c_int64),
+                ("stride_col_base", ctypes.c_int64), ("stride_col_dst", ctypes.c_int64),
+                ("stride_a_slot", ctypes.c_int64), ("stride_a_row", ctypes.c_int64),
+                ("stride_b_slot", ctypes.c_int64), ("stride_b_row", ctypes.c_int64), ("slots", ctypes.c_int),
+                ("rank", ctypes.c_int), ("type", ctypes.c_int)]
+
+
+class RopeTensor(ctypes.Structure):
+    """struct q4k_rope_tensor (include/q4k_gemv.h)."""
+    _fields_ = [("x", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("stride_col_x", ctypes.c_int64),
+                ("stride_head_x", ctypes.c_int64), ("stride_col_dst", ctypes.c_int64),
+                ("stride_head_dst", ctypes.c_int64), ("heads", ctypes.c_int)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """struct q4k_logits_args (include/q4k_gemv.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("nvocab", ctypes.c_int64),
+                ("stride_col", ctypes.c_int64), ("stride_col_dst", ctypes.c_int64), ("history", ctypes.c_void_p),
+                ("history_len", ctypes.c_void_p), ("penalties", ctypes.c_void_p), ("max_history", ctypes.c_int64),
+                ("stride_history", ctypes.c_int64), ("bias_tokens", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("bias_offsets", ctypes.c_void_p), ("n_bias", ctypes.c_int64),
+                ("mask", ctypes.c_void_p), ("mask_rows", ctypes.c_void_p), ("stride_mask", ctypes.c_int64),
+                ("n_masks", ctypes.c_int), ("token", ctypes.c_void_p), ("lse", ctypes.c_void_p)]
+
+
 # Q4K_GLU_* (include/q4k_gemv.h)
 GLU_NONE, GLU_SWIGLU, GLU_GEGLU, GLU_SWIGLU_OAI, GLU_MUL = 0, 1, 2, 3, 4
 GLU_OPS = {"none": GLU_NONE, "swiglu": GLU_SWIGLU, "geglu": GLU_GEGLU, "swiglu_oai": GLU_SWIGLU_OAI,
@@ -145,6 +174,11 @@ def lib() -> ctypes.CDLL:
             "q4k_ipc_close": (None, [_P]),
             "q4k_batch_ex_kernel": (_I, [TXP, _I, _I, _I]),
             "q4k_batch_persistent_kernel": (_I, [TP, _I, _I, _I]),
+            "q4k_lora_workspace_bytes": (_SZ, [ctypes.POINTER(LoraTask), _I, _I]),
+            "q4k_lora_batch": (None, [ctypes.POINTER(LoraTask), _I, _I, _P, _P, _SZ, _P]),
+            "q4k_rope_multi": (None, [ctypes.POINTER(RopeTensor), _I, _I, _I, _I, _P, _I64, _P, ctypes.POINTER(_I),
+                                      _I, _I, _I, ctypes.c_float, _I, _P]),
+            "q4k_logits_process": (None, [ctypes.POINTER(LogitsArgs), _I, _P]),
             "q4k_timeline_bytes": (_SZ, []),
             "q4k_timeline_read": (None, [_P, _SZ, ctypes.POINTER(_I)]),
             "q4k_timeline_reset": (None, []),
@@ -556,6 +590,268 @@ def debug_subblock_sums(W, yq, K: int, ws: Workspace | None = None, stream=None)
                                          W.stride(0) // BLOCK_BYTES, yq.stride(0) // Q8_1_BYTES,
                                          S.data_ptr(), T.data_ptr(), w.ptr, w.nbytes, _stream(stream)))
     return S, T
+
+
+# ---------------------------------------------------------------------------
+# what each request of a batch brings of its own: adapters, positions, controls
+# ---------------------------------------------------------------------------
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30  # Q4K_TYPE_*: ggml's type numbers
+ROPE_LAYOUTS = {"half": 0, "adjacent": 1}
+ROPE_ORDERS = {"blocks": 0, "interleaved": 1}
+
+
+def _type_of(dtype) -> int:
+    import torch
+    t = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}.get(dtype)
+    if t is None:
+        raise Q4KError(1, f"type {dtype} is not float32, float16 or bfloat16")
+    return t
+
+
+def _dense(t, name: str, ndim: int, dtype, device):
+    """t, checked: on `device`, of `dtype` (None: any) and `ndim` dimensions, the last one contiguous."""
+    if t.dim() != ndim or t.device != device or (dtype is not None and t.dtype != dtype):
+        raise Q4KError(1, f"{name}: {ndim}-d {dtype or 'tensor'} on {device} expected, got {tuple(t.shape)} "
+                          f"{t.dtype} on {t.device}")
+    if ndim and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise Q4KError(1, f"{name}: the last dimension is not contiguous")
+    return t
+
+
+def _flat(t, name: str, dtype, n: int, device) -> int | None:
+    """Address of a contiguous 1-d tensor of n values (None stays None)."""
+    if t is None:
+        return None
+    if t.shape != (n,):
+        raise Q4KError(1, f"{name}: {n} values expected, got {tuple(t.shape)}")
+    return _dense(t, name, 1, dtype, device).data_ptr()
+
+
+def _on_cuda(t, name: str):
+    if not t.is_cuda:
+        raise Q4KError(1, f"{name}: not a CUDA tensor (there is no CPU fallback)")
+    return t.device
+
+
+def _new(shape, dtype, device, stream):
+    """An uninitialised tensor that belongs to the stream the call runs on."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _call_on(device, stream, fn, *args) -> int:
+    """fn(*args, stream) with the tensors' device current; stream None: that device's current one."""
+    import torch
+    s = torch.cuda.current_stream(device).cuda_stream if stream is None else _stream(stream)
+    if device.index == torch.cuda.current_device():
+        return fn(*args, s)
+    with torch.cuda.device(device):
+        return fn(*args, s)
+
+
+def _lora_fill(t: LoraTask, it: dict, stream):
+    """One q4k_lora_task from a dict; returns (output, ncols, device)."""
+    import torch
+    x, A, B, base, out = it["x"], it["A"], it["B"], it.get("base"), it.get("out")
+    dev = _on_cuda(x, "x")
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    ncols, K = _dense(x, "x", 2, torch.float32, dev).shape
+    slots, rank, ka = _dense(A, "A", 3, None, dev).shape
+    sb, nrows, rb = _dense(B, "B", 3, A.dtype, dev).shape
+    if ka != K or sb != slots or rb != rank:
+        raise Q4KError(1, f"A {tuple(A.shape)} and B {tuple(B.shape)} do not fit x {tuple(x.shape)}")
+    t.type = _type_of(A.dtype)
+    if out is None:
+        out = _new((ncols, nrows), torch.float32, dev, stream)
+    o = out.unsqueeze(0) if out.dim() == 1 else out
+    if _dense(o, "out", 2, torch.float32, dev).shape != (ncols, nrows):
+        raise Q4KError(1, f"out {tuple(out.shape)}: ({ncols}, {nrows}) expected")
+    if base is not None:
+        b = base.unsqueeze(0) if base.dim() == 1 else base
+        if _dense(b, "base", 2, torch.float32, dev).shape != (ncols, nrows):
+            raise Q4KError(1, f"base {tuple(base.shape)}: ({ncols}, {nrows}) expected")
+        t.base, t.stride_col_base = b.data_ptr(), b.stride(0)
+    t.x, t.A, t.B, t.dst = x.data_ptr(), A.data_ptr(), B.data_ptr(), o.data_ptr()
+    t.ranks = _flat(it.get("ranks"), "ranks", torch.int32, slots, dev)
+    t.scales = _flat(it.get("scales"), "scales", torch.float32, slots, dev)
+    t.K, t.nrows, t.slots, t.rank = K, nrows, slots, rank
+    t.stride_col_x, t.stride_col_dst = x.stride(0), o.stride(0)
+    t.stride_a_slot, t.stride_a_row = A.stride(0), A.stride(1)
+    t.stride_b_slot, t.stride_b_row = B.stride(0), B.stride(1)
+    return out, ncols, dev
+
+
+def make_lora_tasks(items: Sequence):
+    """ctypes q4k_lora_task array for lora_batch from dicts with keys x (ncols, K) fp32,
+    A (slots, rank, K) and B (slots, nrows, rank) of one type (fp32, fp16 or bf16), out
+    (ncols, nrows) and optionally base (fp32 like out, may be out itself), ranks (slots
+    int32) and scales (slots fp32).  The tensors must outlive the array."""
+    arr = (LoraTask * len(items))()
+    for t, it in zip(arr, items):
+        if it.get("out") is None:
+            raise Q4KError(1, "make_lora_tasks: an item has no out")
+        _lora_fill(t, it, None)
+    return arr
+
+
+def _lora_call(arr, ncols: int, ids, dev, ws, stream) -> None:
+    import torch
+    idp = _flat(ids, "ids", torch.int32, ncols, dev)
+    fn, n = lib().q4k_lora_batch, len(arr)
+    st = _call_on(dev, stream, fn, arr, n, ncols, idp, ws.ptr if ws is not None else None,
+                  ws.nbytes if ws is not None else 0)
+    if st == 5:
+        need = int(lib().q4k_lora_workspace_bytes(arr, n, ncols))
+        if ws is not None:
+            ws.ensure(need)
+            p = ws.ptr
+        else:  # scratch of this call's own, so calls on several streams or in several graphs share nothing
+            scratch = _new((need,), torch.uint8, dev, stream)
+            p = scratch.data_ptr()
+        st = _call_on(dev, stream, fn, arr, n, ncols, idp, p, need)
+    _check(st)
+
+
+def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
+    """Low-rank adapters of many requests beside the projections of a step:
+    out[j] = base[j] + scales[a] * B[a] @ (A[a] @ x[j]) with a = ids[j] (int32 on the
+    device, one per column, the same for all tasks; outside 0..slots-1, e.g. -1: no
+    adapter, out[j] = base[j]).  tasks: dicts as for make_lora_tasks (out may be left
+    out), returns the list of outputs; or its array, returns None."""
+    if isinstance(tasks, ctypes.Array):
+        _lora_call(tasks, ids.shape[0], ids, _on_cuda(ids, "ids"), ws, stream)
+        return None
+    if len(tasks) == 0:
+        return []
+    arr = (LoraTask * len(tasks))()
+    got = [_lora_fill(t, it, stream) for t, it in zip(arr, tasks)]
+    if any(g[1:] != got[0][1:] for g in got):
+        raise Q4KError(1, "the tasks' columns or devices differ")
+    _lora_call(arr, got[0][1], ids, got[0][2], ws, stream)
+    return [g[0] for g in got]
+
+
+def lora_add(x, A, B, ids, base=None, ranks=None, scales=None, out=None, ws: Workspace | None = None, stream=None):
+    """lora_batch for one projection; returns (ncols, nrows) fp32."""
+    t = (LoraTask * 1)()
+    out, ncols, dev = _lora_fill(t[0], dict(x=x, A=A, B=B, base=base, ranks=ranks, scales=scales, out=out), stream)
+    _lora_call(t, ncols, ids, dev, ws, stream)
+    return out
+
+
+def rope_inv_freq(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, factors=None, device=None):
+    """Angle per position step of the n_rot/2 rotary pairs, fp64 on the device:
+    freq_scale * freq_base^(-2i/n_rot), divided by factors[i] where given."""
+    import torch
+    i = torch.arange(n_rot // 2, dtype=torch.float64)
+    f = float(freq_scale) * float(freq_base) ** (-2.0 * i / max(1, n_rot))
+    if factors is not None:
+        f = f / torch.as_tensor(factors).to("cpu", torch.float64)
+    return f.to("cuda" if device is None else device)
+
+
+def rope_multi(x, pos, inv_freq, sections, layout: str = "half", order: str = "blocks", scale: float = 1.0,
+               dtype=None, out=None, stream=None):
+    """Rotary positions with several axes.  x: (ncols, heads, head_dim) fp32, or a sequence of
+    up to 4 such tensors (queries and keys) turned by one launch; pos: (axes, ncols) int32;
+    inv_freq: (n_rot/2) fp64 (rope_inv_freq); sections: pairs per axis.  layout: "half" pairs
+    (i, i + n_rot/2), "adjacent" (2i, 2i+1); order: "blocks" or "interleaved" axes
+    (include/q4k_gemv.h).  out: tensor(s) like x, x itself to turn in place, or None (new, of
+    `dtype`: fp32, fp16 or bf16).  Returns out."""
+    import torch
+    single = not isinstance(x, (list, tuple))
+    xs = [x] if single else list(x)
+    if layout not in ROPE_LAYOUTS or order not in ROPE_ORDERS:
+        raise Q4KError(1, f"layout {layout!r} / order {order!r}")
+    outs = [None] * len(xs) if out is None else [out] if single else list(out)
+    if not 1 <= len(xs) <= 4 or len(outs) != len(xs):
+        raise Q4KError(1, "1 to 4 tensors, and as many outputs")
+    dev = _on_cuda(xs[0], "x")
+    ncols, _, dim = xs[0].shape if xs[0].dim() == 3 else (0, 0, 0)
+    if dtype is None:
+        dtype = outs[0].dtype if outs[0] is not None else torch.float32
+    arr = (RopeTensor * len(xs))()
+    for i, (t, v) in enumerate(zip(arr, xs)):
+        _dense(v, "x", 3, torch.float32, dev)
+        if outs[i] is None:
+            outs[i] = _new(v.shape, dtype, dev, stream)
+        o = _dense(outs[i], "out", 3, dtype, dev)
+        if o.shape != v.shape or v.shape[0] != ncols or v.shape[2] != dim:
+            raise Q4KError(1, f"x {tuple(v.shape)}, out {tuple(o.shape)}: ({ncols}, heads, {dim}) expected")
+        t.x, t.dst, t.heads = v.data_ptr(), o.data_ptr(), v.shape[1]
+        t.stride_col_x, t.stride_head_x = v.stride(0), v.stride(1)
+        t.stride_col_dst, t.stride_head_dst = o.stride(0), o.stride(1)
+    _dense(pos, "pos", 2, torch.int32, dev)
+    _dense(inv_freq, "inv_freq", 1, torch.float64, dev)
+    if pos.shape != (len(sections), ncols):
+        raise Q4KError(1, f"pos {tuple(pos.shape)}: ({len(sections)}, {ncols}) expected")
+    sect = (_I * len(sections))(*sections)
+    _check(_call_on(dev, stream, lib().q4k_rope_multi, arr, len(xs), ncols, dim, 2 * inv_freq.shape[0],
+                    pos.data_ptr(), pos.stride(0), inv_freq.data_ptr(), sect, len(sections), ROPE_ORDERS[order],
+                    ROPE_LAYOUTS[layout], scale, _type_of(dtype)))
+    return outs[0] if single else outs
+
+
+def logits_process(logits, history=None, history_len=None, penalties=None, bias_tokens=None, bias_values=None,
+                   bias_offsets=None, mask=None, mask_rows=None, out=None, pick: bool = False, stream=None):
+    """Penalties for repeated tokens, biases and masks on logits (ncols, nvocab) fp32, per
+    column: history (ncols, max_history) int32 with history_len (ncols) and penalties
+    (ncols, 3) = {repeat, frequency, presence}; bias entries bias_offsets[j]..bias_offsets[j+1]
+    of bias_tokens (int32) / bias_values (fp32), duplicates added up; row mask_rows[j] (others
+    than an existing row, e.g. -1: none) of the bit mask (n_masks, ceil(nvocab/32)) int32 or
+    uint32, bit set = allowed, else -inf.  out may be logits itself.  Returns out; with
+    pick=True (out, token, lse): the lowest index of the largest value (-1: nothing left) and
+    log(sum(exp)) of every column."""
+    import torch
+    dev = _on_cuda(logits, "logits")
+    lg = logits.unsqueeze(0) if logits.dim() == 1 else logits
+    ncols, nvocab = _dense(lg, "logits", 2, torch.float32, dev).shape
+    if out is None:
+        out = _new(logits.shape, torch.float32, dev, stream)
+    o = out.unsqueeze(0) if out.dim() == 1 else out
+    if _dense(o, "out", 2, torch.float32, dev).shape != lg.shape:
+        raise Q4KError(1, f"out {tuple(out.shape)}: {tuple(logits.shape)} expected")
+    if (history is None) != (penalties is None) or (history is None and history_len is not None):
+        raise Q4KError(1, "history and penalties go together")
+    if (bias_tokens is None) != (bias_values is None) or (bias_tokens is None) != (bias_offsets is None):
+        raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
+    if mask is None and mask_rows is not None:
+        raise Q4KError(1, "mask_rows without a mask")
+    a = LogitsArgs()
+    a.logits, a.dst, a.nvocab, a.stride_col, a.stride_col_dst = lg.data_ptr(), o.data_ptr(), nvocab, lg.stride(0), \
+        o.stride(0)
+    if history is not None:
+        if history.shape[0] != ncols:
+            raise Q4KError(1, f"history {tuple(history.shape)}: {ncols} rows expected")
+        a.history = _dense(history, "history", 2, torch.int32, dev).data_ptr()
+        a.max_history, a.stride_history = history.shape[1], history.stride(0)
+        a.history_len = _flat(history_len, "history_len", torch.int32, ncols, dev)
+        if penalties.shape != (ncols, 3) or not penalties.is_contiguous():
+            raise Q4KError(1, f"penalties {tuple(penalties.shape)}: ({ncols}, 3) contiguous expected")
+        a.penalties = _dense(penalties, "penalties", 2, torch.float32, dev).data_ptr()
+    if bias_tokens is not None:
+        a.n_bias = bias_tokens.shape[0]
+        a.bias_tokens = _flat(bias_tokens, "bias_tokens", torch.int32, a.n_bias, dev)
+        a.bias_values = _flat(bias_values, "bias_values", torch.float32, a.n_bias, dev)
+        a.bias_offsets = _flat(bias_offsets, "bias_offsets", torch.int32, ncols + 1, dev)
+    if mask is not None:
+        _dense(mask, "mask", 2, None, dev)
+        if mask.dtype not in (torch.int32, torch.uint32) or mask.shape[1] != (nvocab + 31) // 32:
+            raise Q4KError(1, f"mask {tuple(mask.shape)} {mask.dtype}: (masks, {(nvocab + 31) // 32}) int32 expected")
+        a.mask, a.n_masks, a.stride_mask = mask.data_ptr(), mask.shape[0], mask.stride(0)
+        a.mask_rows = _flat(mask_rows, "mask_rows", torch.int32, ncols, dev)
+    token = lse = None
+    if pick:
+        token, lse = _new((ncols,), torch.int32, dev, stream), _new((ncols,), torch.float32, dev, stream)
+        a.token, a.lse = token.data_ptr(), lse.data_ptr()
+    _check(_call_on(dev, stream, lib().q4k_logits_process, ctypes.byref(a), ncols))
+    return (out, token, lse) if pick else out
 
 
 # ---------------------------------------------------------------------------

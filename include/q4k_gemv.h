@@ -371,6 +371,124 @@ Q4K_API int q4k_mul_mat_vec_noalloc(const void *W, const float *x, float *dst,
 /* Size of that built-in scratch array in bytes. */
 Q4K_API size_t q4k_noalloc_scratch_bytes(void);
 
+/* ---- what each request of a batch brings of its own ----------------------------- */
+
+/* A batch's columns share the weights above; three things belong to the
+ * request behind each column: its low-rank adapter, its rotary positions and
+ * the controls on its logits.  The entries below take these as device arrays
+ * indexed by column, so one captured graph serves changing requests.  No
+ * counterpart in the reference (upstream llama.cpp runs them as separate graph
+ * nodes or on the host).  They take any number of columns (ncols 0: nothing
+ * to do), keep nothing between calls and give the same bits every time. */
+
+/* Element types of adapters and outputs (ggml's type numbers). */
+#define Q4K_TYPE_F32 0
+#define Q4K_TYPE_F16 1
+#define Q4K_TYPE_BF16 30
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   dst[j][n] = base[j][n] + scales[a] * sum_{t < ranks[a]} B[a][n][t] * (sum_k A[a][t][k] * x[j][k]),
+ * a = ids[j], the adapter slot of column j; an id outside 0..slots-1 (by
+ * convention -1) means no adapter: dst[j] = base[j].  All sums are fp32.
+ * x, base and dst are fp32 columns as in q4k_task (base usually the GEMV's
+ * dst).  A holds `slots` matrices of rank x K, B of nrows x rank; strides are
+ * in elements, the innermost dimension is contiguous. */
+typedef struct q4k_lora_task {
+    const float *x;          /* K x ncols, column stride stride_col_x */
+    const float *base;       /* nrows x ncols, or NULL (zeros); may be dst itself (same stride) */
+    float *dst;              /* nrows x ncols; overlaps neither x nor another task's dst */
+    const void *A;           /* down projections */
+    const void *B;           /* up projections */
+    const int32_t *ranks;    /* slots ranks, clamped to 0..rank; NULL: all are rank */
+    const float *scales;     /* slots factors; NULL: all are 1 */
+    int64_t K;
+    int64_t nrows;
+    int64_t stride_col_x;    /* >= K, or 0: one column for all */
+    int64_t stride_col_base; /* >= nrows, or 0: one column for all (unused without base) */
+    int64_t stride_col_dst;  /* >= nrows */
+    int64_t stride_a_slot;   /* any, not negative */
+    int64_t stride_a_row;    /* >= K */
+    int64_t stride_b_slot;   /* any, not negative */
+    int64_t stride_b_row;    /* >= rank */
+    int slots;               /* adapter slots, 0..Q4K_MAX_LORA_SLOTS */
+    int rank;                /* rank the slots have room for, 0..Q4K_MAX_LORA_RANK */
+    int type;                /* Q4K_TYPE_* of A and B */
+} q4k_lora_task;
+
+#define Q4K_MAX_LORA_SLOTS 1024
+#define Q4K_MAX_LORA_RANK 512
+/* Every task's adapters for all columns; ids (ncols device ints) serves all
+ * tasks (at most Q4K_MAX_TASKS).  The workspace need not be initialised. */
+Q4K_API size_t q4k_lora_workspace_bytes(const q4k_lora_task *tasks, int ntasks, int ncols);
+Q4K_API int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int32_t *ids, void *workspace,
+                           size_t workspace_bytes, q4k_stream_t stream);
+
+/* Rotary positions with several axes (time, height, width, ...) on up to
+ * Q4K_MAX_ROPE_TENSORS tensors of one step (queries and keys).  Pair i of the
+ * n_rot/2 rotated pairs of every head of column j turns by
+ *   phi = pos[axis(i)][j] * inv_freq[i]     (formed and reduced in fp64):
+ *   (x_a, x_b) -> scale * (x_a cos phi - x_b sin phi, x_b cos phi + x_a sin phi),
+ * with (a, b) = (i, i + n_rot/2) for Q4K_ROPE_HALF and (2i, 2i+1) for
+ * Q4K_ROPE_ADJACENT; values from n_rot on are copied.  axis(i):
+ *   Q4K_ROPE_BLOCKS       sections[0] pairs of axis 0, then sections[1] of
+ *                         axis 1, ..., from the start again after the last
+ *                         (sections must not all be 0);
+ *   Q4K_ROPE_INTERLEAVED  axes in turn, i mod n_axes, while i / n_axes is below
+ *                         that axis's section; the other pairs: axis 0.
+ * Positions may be negative (a shift of cached keys back). */
+#define Q4K_ROPE_HALF 0
+#define Q4K_ROPE_ADJACENT 1
+#define Q4K_ROPE_BLOCKS 0
+#define Q4K_ROPE_INTERLEAVED 1
+#define Q4K_MAX_ROPE_TENSORS 4
+#define Q4K_MAX_ROPE_AXES 4
+#define Q4K_MAX_ROPE_DIM 1024
+typedef struct q4k_rope_tensor {
+    const float *x;          /* heads of head_dim contiguous values */
+    void *dst;               /* of dst_type; may be x itself (fp32, same strides), else must not overlap */
+    int64_t stride_col_x;    /* elements between columns */
+    int64_t stride_head_x;   /* elements between heads (>= head_dim) */
+    int64_t stride_col_dst;
+    int64_t stride_head_dst;
+    int heads;
+} q4k_rope_tensor;
+Q4K_API int q4k_rope_multi(const q4k_rope_tensor *tensors, int ntensors, int ncols, int head_dim, int n_rot,
+                           const int32_t *pos, int64_t stride_axis_pos, const double *inv_freq, const int *sections,
+                           int n_axes, int order, int layout, float scale, int dst_type, q4k_stream_t stream);
+
+/* Penalties for repeated tokens, biases and masks on the head's logits, with
+ * the greedy token and the log-sum-exp of the result from the same pass.  Per
+ * column j and token v, in fp32:
+ *   z = logits[j][v] + sum of the biases of column j at v, added up first, in list order;
+ *   if v occurs c > 0 times in the history of column j:
+ *       z = z > 0 ? z / repeat : z * repeat;  z = z - (c * frequency + presence);
+ *   if column j's mask has bit v clear: z = -inf, whatever z was.
+ * token[j]: the lowest index with the largest z above -inf (NaN is never
+ * picked), or -1; lse[j] = log(sum_v exp(z)): -inf when nothing is left. */
+typedef struct q4k_logits_args {
+    const float *logits;          /* nvocab x ncols, column stride stride_col */
+    float *dst;                   /* may be logits itself (same stride), else must not overlap */
+    int64_t nvocab;
+    int64_t stride_col;           /* >= nvocab, or 0: one column for all */
+    int64_t stride_col_dst;       /* >= nvocab */
+    const int32_t *history;       /* max_history x ncols tokens (others than 0..nvocab-1: ignored), or NULL */
+    const int32_t *history_len;   /* entries used per column, clamped to 0..max_history; NULL: all */
+    const float *penalties;       /* per column {repeat, frequency, presence}; goes with history */
+    int64_t max_history;
+    int64_t stride_history;       /* >= max_history, or 0: one history for all */
+    const int32_t *bias_tokens;   /* n_bias tokens (others than 0..nvocab-1: ignored), or NULL */
+    const float *bias_values;     /* n_bias values */
+    const int32_t *bias_offsets;  /* ncols + 1: column j's entries are [offsets[j], offsets[j+1]), clamped to 0..n_bias */
+    int64_t n_bias;
+    const uint32_t *mask;         /* n_masks rows of ceil(nvocab/32) words, bit v%32 of word v/32: allowed; or NULL */
+    const int32_t *mask_rows;     /* mask row per column; outside 0..n_masks-1: no mask.  NULL: column j uses row j */
+    int64_t stride_mask;          /* words between mask rows */
+    int n_masks;
+    int32_t *token;               /* ncols, or NULL */
+    float *lse;                   /* ncols, or NULL */
+} q4k_logits_args;
+Q4K_API int q4k_logits_process(const q4k_logits_args *args, int ncols, q4k_stream_t stream);
+
 /* ---- diagnostics ------------------------------------------------------------- */
 
 /* Which GEMV kernel q4k_gemv_batch_ex (or q4k_gemv_batch) would run for these
