@@ -5,10 +5,14 @@
 //   dst[j][n] = base[j][n] + sum_t B_a[n][t] u[j][t]     (expand), a = ids[j]
 #include "q4k_request.h"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 using namespace q4k;
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -82,8 +86,259 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
     }
 }
 
+// ---- few columns: one cluster per adapter and group of columns -------------------
+// The A and B of a column's adapter are the bytes of the call (1 MB at rank 64,
+// 4096 x 4096, 16 bits), and a step's calls are too short for two launches. One
+// launch: the cluster splits K over its CTAs (each reads its slice of every row
+// of A once), the partial u meet over distributed shared memory, and each CTA
+// expands its slice of the rows of B. Columns that share an adapter share the
+// reading: the cluster of every kGroup-th column of an adapter takes the next
+// kGroup of them, the clusters of the others end at once.
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGroup = 8;    // columns of one adapter per cluster
+constexpr int kTile = 1024;  // values of x per column in shared memory at a time
+constexpr int kClusterCols = 64;  // columns up to which the cluster kernel runs
+constexpr int kBatch = 4;    // rows of A or B in flight per lane
+
+// V values of T as they lie in memory; V * sizeof(T) is 16 (one load) or V is 1.
+template <typename T, int V> struct alignas(V > 1 ? 16 : sizeof(T)) Chunk {
+    T v[V];
+};
+template <typename T, int V> __device__ __forceinline__ Chunk<T, V> zero_chunk() {
+    Chunk<T, V> c;
+#pragma unroll
+    for (int e = 0; e < V; ++e) c.v[e] = T(0.0f);
+    return c;
+}
+// Values [0, n) of a row at p, n >= 1; the rest is zero and not read.
+template <typename T, int V> __device__ __forceinline__ Chunk<T, V> load_chunk(const T *p, int n) {
+    if constexpr (V > 1) {
+        if (n >= V) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
+            return *reinterpret_cast<const Chunk<T, V> *>(&raw);
+        }
+        Chunk<T, V> c = zero_chunk<T, V>();
+#pragma unroll
+        for (int e = 0; e < V - 1; ++e)
+            if (e < n) c.v[e] = p[e];
+        return c;
+    } else {
+        Chunk<T, V> c;
+        c.v[0] = __ldg(p);
+        return c;
+    }
+}
+
+// The columns of one group, G of them in registers (count <= G of them real).
+template <typename T, int VA, int VB, int G>
+__device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, int count, const int *cols, float *xs,
+                                           float *part, float *us, cg::cluster_group &cluster) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int nc = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
+    // shrink: this CTA's slice of K
+    const int kper = ((t.K + nc - 1) / nc + 7) / 8 * 8;
+    const int k0 = min(t.K, me * kper), k1 = min(t.K, k0 + kper);
+    for (int i = tid; i < r * G; i += kThreads) part[i] = 0.0f;
+    const T *A = static_cast<const T *>(t.A) + a * t.sa_slot;
+    for (int sub = k0; sub < k1; sub += kTile) {
+        const int kt = min(kTile, k1 - sub);
+        __syncthreads();
+        for (int i = tid; i < kt; i += kThreads)
+#pragma unroll
+            for (int g = 0; g < G; ++g) xs[g * kTile + i] = g < count ? t.x[cols[g] * t.sx + sub + i] : 0.0f;
+        __syncthreads();
+        for (int t0 = warp; t0 < r; t0 += kWarps * kBatch) {
+            float acc[kBatch][G] = {};
+            for (int c = lane * VA; c < kt; c += 32 * VA) {
+                Chunk<T, VA> w[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int q = t0 + i * kWarps;
+                    w[i] = q < r ? load_chunk<T, VA>(A + q * t.sa_row + sub + c, kt - c) : zero_chunk<T, VA>();
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+#pragma unroll
+                    for (int e = 0; e < VA; ++e) {
+                        // (a chunk's tail holds zeros of A; x behind the tile is not read into it)
+                        const float x = VA == 1 || c + e < kt ? xs[g * kTile + c + e] : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < kBatch; ++i) acc[i][g] = fmaf(to_f32(w[i].v[e]), x, acc[i][g]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float s = acc[i][g];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                    if (lane == 0 && t0 + i * kWarps < r) part[(t0 + i * kWarps) * G + g] += s;
+                }
+            }
+        }
+    }
+    // expand: L lanes per row of B, kBatch rows in flight; the first rows are asked for before the barrier
+    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
+    const int nper = (t.nrows + nc - 1) / nc;
+    const int n0 = min(t.nrows, me * nper), n1 = min(t.nrows, n0 + nper);
+    int L = 1;
+    while (L < 32 && L * VB < r) L *= 2;
+    const int sub = lane & (L - 1), row = warp * (32 / L) + lane / L, step = kThreads / L;
+    Chunk<T, VB> w[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int n = n0 + row + i * step;
+        w[i] = n < n1 && sub * VB < r ? load_chunk<T, VB>(B + n * t.sb_row + sub * VB, r - sub * VB)
+                                      : zero_chunk<T, VB>();
+    }
+    cluster.sync();
+    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
+    for (int i = tid; i < r * G; i += kThreads) {
+        float s = 0.0f;
+        for (int c = 0; c < nc; ++c) s += cluster.map_shared_rank(part, c)[i];
+        us[i] = s * scale;
+    }
+    __syncthreads();
+    for (int nb = n0; nb < n1; nb += kBatch * step) {
+        float acc[kBatch][G] = {};
+        for (int c = sub * VB;; c += L * VB) {
+            if (nb > n0 || c >= L * VB) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int n = nb + row + i * step;
+                    w[i] = n < n1 && c < r ? load_chunk<T, VB>(B + n * t.sb_row + c, r - c) : zero_chunk<T, VB>();
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VB; ++e) {
+                if (c + e < r) {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float u = us[(c + e) * G + g];
+#pragma unroll
+                        for (int i = 0; i < kBatch; ++i) acc[i][g] = fmaf(to_f32(w[i].v[e]), u, acc[i][g]);
+                    }
+                }
+            }
+            if (c - sub * VB + L * VB >= r) break;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int n = nb + row + i * step;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float s = acc[i][g];
+                for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (g < count && n < n1 && sub == (g & (L - 1))) {
+                    const float b = t.base != nullptr ? t.base[cols[g] * t.sbase + n] : 0.0f;
+                    t.dst[cols[g] * t.sdst + n] = b + s;
+                }
+            }
+        }
+    }
+    cluster.sync();  // no CTA leaves while another may still read its part
+}
+
+template <typename T, int VA, int VB>
+__global__ void __launch_bounds__(kThreads) k_lora_cluster(const __grid_constant__ LoraParams P) {
+    extern __shared__ __align__(16) float smem[];
+    __shared__ int cols[kGroup];
+    __shared__ int found;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int nc = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
+    const LoraTask &t = P.task[blockIdx.y];
+    const int j = blockIdx.x / nc;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int a = slot_of(t, P.ids[j]);
+    const int r = a < 0 ? 0 : rank_of(t, a);
+    if (r == 0) {  // nothing to add: the column's rows are base's
+        const int nper = (t.nrows + nc - 1) / nc;
+        const int n0 = min(t.nrows, me * nper), n1 = min(t.nrows, n0 + nper);
+        for (int n = n0 + tid; n < n1; n += kThreads)
+            t.dst[j * t.sdst + n] = t.base != nullptr ? t.base[j * t.sbase + n] : 0.0f;
+        return;  // (the whole cluster takes this way)
+    }
+    if (tid < 32) {
+        int before = 0;
+        for (int i = lane; i < j; i += 32) before += slot_of(t, P.ids[i]) == a;
+        before = __reduce_add_sync(0xffffffffu, before);
+        int n = 0;
+        if (before % kGroup == 0) {
+            for (int i0 = j; i0 < P.ncols && n < kGroup; i0 += 32) {
+                const unsigned m = __ballot_sync(0xffffffffu, i0 + lane < P.ncols && P.ids[min(i0 + lane, P.ncols - 1)] == a);
+                const int at = n + __popc(m & ((1u << lane) - 1));
+                if (((m >> lane) & 1u) && at < kGroup) cols[at] = i0 + lane;
+                n = min(kGroup, n + __popc(m));
+            }
+        }
+        if (lane == 0) found = n;
+    }
+    __syncthreads();
+    const int count = found;
+    if (count == 0) return;  // another column's cluster does this one (all CTAs agree)
+    float *xs = smem, *part = smem + kGroup * kTile, *us = part + kGroup * t.rank;
+    if (count == 1)
+        lora_group<T, VA, VB, 1>(t, a, r, count, cols, xs, part, us, cluster);
+    else if (count <= 4)
+        lora_group<T, VA, VB, 4>(t, a, r, count, cols, xs, part, us, cluster);
+    else
+        lora_group<T, VA, VB, kGroup>(t, a, r, count, cols, xs, part, us, cluster);
+}
+
+size_t cluster_smem(int rank) { return (kGroup * kTile + 2 * kGroup * rank) * sizeof(float); }
+
+template <typename T, int VA, int VB>
+cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
+    auto *fn = k_lora_cluster<T, VA, VB>;
+    static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem(Q4K_MAX_LORA_RANK));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    }
+    const int nc = 16;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.ncols * nc, ntasks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = cluster_smem(rank);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = nc;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+// Whether chunks of V values of every row are 16-byte aligned.
+bool rows_aligned(const void *p, int64_t slot, int64_t row, int esz) {
+    return aligned_to(p, 16) && slot * esz % 16 == 0 && row * esz % 16 == 0;
+}
+
 template <typename T>
 cudaError_t launch_lora(const LoraParams &p, int ntasks, cudaStream_t s) {
+    if (p.ncols <= kClusterCols) {
+        constexpr int V = 16 / sizeof(T);
+        bool va = true, vb = true;
+        int rank = 0;
+        for (int i = 0; i < ntasks; ++i) {
+            const LoraTask &t = p.task[i];
+            va = va && rows_aligned(t.A, t.sa_slot, t.sa_row, sizeof(T));
+            vb = vb && rows_aligned(t.B, t.sb_slot, t.sb_row, sizeof(T));
+            rank = t.rank > rank ? t.rank : rank;
+        }
+        return va ? vb ? launch_cluster<T, V, V>(p, ntasks, rank, s) : launch_cluster<T, V, 1>(p, ntasks, rank, s)
+                  : vb ? launch_cluster<T, 1, V>(p, ntasks, rank, s) : launch_cluster<T, 1, 1>(p, ntasks, rank, s);
+    }
     k_lora_shrink<T><<<dim3(p.ncols, ntasks), 256, 0, s>>>(p);
     k_lora_expand<T><<<dim3(p.ncols, ntasks, 8), 256, 0, s>>>(p);
     return cudaGetLastError();
@@ -167,6 +422,7 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
 }
 
 size_t workspace_need(const q4k_lora_task *tasks, int ntasks, int ncols) {
+    if (ncols <= kClusterCols) return 0;
     size_t u = 0;
     for (int i = 0; i < ntasks; ++i)
         if (tasks[i].nrows > 0) u += static_cast<size_t>(tasks[i].rank);
