@@ -94,12 +94,20 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
 // expands its slice of the rows of B. Columns that share an adapter share the
 // reading: the cluster of every kGroup-th column of an adapter takes the next
 // kGroup of them, the clusters of the others end at once.
-constexpr int kThreads = 256;
+// What bounds it is the chain of round trips to memory, so it is kept short:
+// ids -> {ranks, scales, x, first A, first B, base} -> partial sums -> cluster
+// barrier -> the other CTAs' parts -> rows.
+#ifndef LORA_T
+#define LORA_T 512
+#define LORA_MB 1
+#endif
+constexpr int kThreads = LORA_T;
 constexpr int kWarps = kThreads / 32;
-constexpr int kGroup = 8;    // columns of one adapter per cluster
-constexpr int kTile = 1024;  // values of x per column in shared memory at a time
-constexpr int kClusterCols = 64;  // columns up to which the cluster kernel runs
-constexpr int kBatch = 4;    // rows of A or B in flight per lane
+constexpr int kClusterCols = 64;  // columns up to which this kernel runs (bits of a mask)
+constexpr int kGroup = 8;         // columns of one adapter per cluster
+constexpr int kTile = 1024;       // values of x per column in shared memory at a time
+constexpr int kBatch = 2;         // rows of A per warp and pass
+constexpr int kAhead = 4;         // chunks of a row of B in flight per lane
 
 // V values of T as they lie in memory; V * sizeof(T) is 16 (one load) or V is 1.
 template <typename T, int V> struct alignas(V > 1 ? 16 : sizeof(T)) Chunk {
@@ -130,169 +138,203 @@ template <typename T, int V> __device__ __forceinline__ Chunk<T, V> load_chunk(c
     }
 }
 
-// The columns of one group, G of them in registers (count <= G of them real).
-template <typename T, int VA, int VB, int G>
-__device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, int count, const int *cols, float *xs,
-                                           float *part, float *us, cg::cluster_group &cluster) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nc = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
-    // shrink: this CTA's slice of K
-    const int kper = ((t.K + nc - 1) / nc + 7) / 8 * 8;
-    const int k0 = min(t.K, me * kper), k1 = min(t.K, k0 + kper);
-    for (int i = tid; i < r * G; i += kThreads) part[i] = 0.0f;
-    const T *A = static_cast<const T *>(t.A) + a * t.sa_slot;
-    for (int sub = k0; sub < k1; sub += kTile) {
-        const int kt = min(kTile, k1 - sub);
-        __syncthreads();
-        for (int i = tid; i < kt; i += kThreads)
+// Sums of M (a power of two, at most 32) values over the warp in M + log2(32 / M) - 1
+// exchanges: each step halves the values a lane still holds. Lane l ends with
+// the sum of value l / (32 / M).
+template <int M> __device__ __forceinline__ float warp_sums(float (&v)[M], int lane) {
+    int o = 16;
 #pragma unroll
-            for (int g = 0; g < G; ++g) xs[g * kTile + i] = g < count ? t.x[cols[g] * t.sx + sub + i] : 0.0f;
-        __syncthreads();
-        for (int t0 = warp; t0 < r; t0 += kWarps * kBatch) {
-            float acc[kBatch][G] = {};
-            for (int c = lane * VA; c < kt; c += 32 * VA) {
-                Chunk<T, VA> w[kBatch];
+    for (int m = M; m > 1; m /= 2, o /= 2) {
+        const bool up = lane & o;
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const int q = t0 + i * kWarps;
-                    w[i] = q < r ? load_chunk<T, VA>(A + q * t.sa_row + sub + c, kt - c) : zero_chunk<T, VA>();
-                }
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-#pragma unroll
-                    for (int e = 0; e < VA; ++e) {
-                        // (a chunk's tail holds zeros of A; x behind the tile is not read into it)
-                        const float x = VA == 1 || c + e < kt ? xs[g * kTile + c + e] : 0.0f;
-#pragma unroll
-                        for (int i = 0; i < kBatch; ++i) acc[i][g] = fmaf(to_f32(w[i].v[e]), x, acc[i][g]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    float s = acc[i][g];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    if (lane == 0 && t0 + i * kWarps < r) part[(t0 + i * kWarps) * G + g] += s;
-                }
-            }
+        for (int i = 0; i < m / 2; ++i) {
+            const float mine = up ? v[i + m / 2] : v[i], other = up ? v[i] : v[i + m / 2];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
         }
     }
-    // expand: L lanes per row of B, kBatch rows in flight; the first rows are asked for before the barrier
-    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
-    const int nper = (t.nrows + nc - 1) / nc;
-    const int n0 = min(t.nrows, me * nper), n1 = min(t.nrows, n0 + nper);
-    int L = 1;
-    while (L < 32 && L * VB < r) L *= 2;
-    const int sub = lane & (L - 1), row = warp * (32 / L) + lane / L, step = kThreads / L;
-    Chunk<T, VB> w[kBatch];
+    float s = v[0];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        const int n = n0 + row + i * step;
-        w[i] = n < n1 && sub * VB < r ? load_chunk<T, VB>(B + n * t.sb_row + sub * VB, r - sub * VB)
-                                      : zero_chunk<T, VB>();
-    }
-    cluster.sync();
-    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
-    for (int i = tid; i < r * G; i += kThreads) {
-        float s = 0.0f;
-        for (int c = 0; c < nc; ++c) s += cluster.map_shared_rank(part, c)[i];
-        us[i] = s * scale;
-    }
-    __syncthreads();
-    for (int nb = n0; nb < n1; nb += kBatch * step) {
-        float acc[kBatch][G] = {};
-        for (int c = sub * VB;; c += L * VB) {
-            if (nb > n0 || c >= L * VB) {
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const int n = nb + row + i * step;
-                    w[i] = n < n1 && c < r ? load_chunk<T, VB>(B + n * t.sb_row + c, r - c) : zero_chunk<T, VB>();
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < VB; ++e) {
-                if (c + e < r) {
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float u = us[(c + e) * G + g];
-#pragma unroll
-                        for (int i = 0; i < kBatch; ++i) acc[i][g] = fmaf(to_f32(w[i].v[e]), u, acc[i][g]);
-                    }
-                }
-            }
-            if (c - sub * VB + L * VB >= r) break;
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int n = nb + row + i * step;
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                float s = acc[i][g];
-                for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (g < count && n < n1 && sub == (g & (L - 1))) {
-                    const float b = t.base != nullptr ? t.base[cols[g] * t.sbase + n] : 0.0f;
-                    t.dst[cols[g] * t.sdst + n] = b + s;
-                }
-            }
-        }
-    }
-    cluster.sync();  // no CTA leaves while another may still read its part
+    for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
 }
 
-template <typename T, int VA, int VB>
-__global__ void __launch_bounds__(kThreads) k_lora_cluster(const __grid_constant__ LoraParams P) {
+// The columns of one group: the lowest G bits of `mask` (fewer where it has fewer).
+template <typename T, int VA, int VB, int G, int NC>
+__device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, uint64_t mask, float *xs, float *part,
+                                           float *us, cg::cluster_group &cluster) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int me = static_cast<int>(cluster.block_rank());
+    int col[G];  // -1: none
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        col[g] = __ffsll(static_cast<long long>(mask)) - 1;
+        mask &= mask - 1;
+    }
+    const T *A = static_cast<const T *>(t.A) + a * t.sa_slot;
+    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
+    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
+
+    // shrink: this CTA's slice [k0, k1) of K, a warp per kBatch rows, the next chunks asked for ahead
+    const int kper = ((t.K + NC - 1) / NC + 7) / 8 * 8;
+    const int k0 = min(t.K, me * kper), k1 = min(t.K, k0 + kper);
+    for (int i = tid; i < r * G; i += kThreads) part[i] = 0.0f;
+    const int passes = (r + kWarps * kBatch - 1) / (kWarps * kBatch);
+
+    // expand: L lanes per row (one where the slice has rows for all threads)
+    const int nper = (t.nrows + NC - 1) / NC;
+    const int n0 = min(t.nrows, me * nper), n1 = min(t.nrows, n0 + nper);
+    int L = 1;
+    while (L < 32 && L * VB < r && 2 * L * nper <= kThreads) L *= 2;
+    const int sub = tid & (L - 1), rows = kThreads / L;
+    int n = n0 + tid / L;
+    Chunk<T, VB> wb[kAhead];
+    float base[G];
+    auto ask = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int c = c0 + i * L * VB;
+            wb[i] = n < n1 && c < r ? load_chunk<T, VB>(B + n * t.sb_row + c, r - c) : zero_chunk<T, VB>();
+        }
+    };
+    auto ask_base = [&]() {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+            base[g] = t.base != nullptr && n < n1 && col[g] >= 0 && sub == (g & (L - 1)) ? t.base[col[g] * t.sbase + n] : 0.0f;
+    };
+
+    for (int k = k0; k < k1; k += kTile) {
+        const int kt = min(kTile, k1 - k);
+        const int chunks = (kt + 32 * VA - 1) / (32 * VA);
+        auto load = [&](Chunk<T, VA> (&w)[kBatch], int pass, int chunk) {
+            const int c = (chunk * 32 + lane) * VA;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int q = pass * kWarps * kBatch + i * kWarps + warp;
+                w[i] = q < r && c < kt ? load_chunk<T, VA>(A + q * t.sa_row + k + c, kt - c) : zero_chunk<T, VA>();
+            }
+        };
+        Chunk<T, VA> w[kBatch];
+        load(w, 0, 0);
+        __syncthreads();  // the tile before this one is done with
+        for (int i = tid; i < chunks * 32 * VA; i += kThreads)  // (zeros where a last chunk reads on)
+#pragma unroll
+            for (int g = 0; g < G; ++g) xs[g * kTile + i] = col[g] >= 0 && i < kt ? t.x[col[g] * t.sx + k + i] : 0.0f;
+        if (k == k0) {
+            ask(sub * VB);
+            ask_base();
+        }
+        __syncthreads();
+        float acc[kBatch * G] = {};
+        for (int pass = 0, chunk = 0; pass < passes;) {
+            const int np = chunk + 1 < chunks ? pass : pass + 1, nx = chunk + 1 < chunks ? chunk + 1 : 0;
+            Chunk<T, VA> next[kBatch];
+            if (np < passes) load(next, np, nx);
+            const int c = (chunk * 32 + lane) * VA;
+#pragma unroll
+            for (int e = 0; e < VA; ++e)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i)
+                        acc[i * G + g] = fmaf(to_f32(w[i].v[e]), xs[g * kTile + c + e], acc[i * G + g]);
+            if (nx == 0) {
+                const float s = warp_sums<kBatch * G>(acc, lane);
+                constexpr int kLanes = 32 / (kBatch * G);
+                const int v = lane / kLanes, q = pass * kWarps * kBatch + v / G * kWarps + warp;
+                if (lane % kLanes == 0 && q < r) part[q * G + v % G] += s;
+#pragma unroll
+                for (int i = 0; i < kBatch * G; ++i) acc[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) w[i] = next[i];
+            pass = np;
+            chunk = nx;
+        }
+    }
+    if (k0 >= k1) {  // (no slice of K here)
+        ask(sub * VB);
+        ask_base();
+    }
+    cluster.sync();
+    for (int i = tid; i < r * G; i += kThreads) {
+        float p[NC], s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) p[c] = cluster.map_shared_rank(part, c)[i];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s += p[c];
+        us[i] = s * scale;
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this CTA has read the others' parts
+    __syncthreads();
+    for (int nb = n0; nb < n1; nb += rows) {  // (uniform: lanes without a row take part in the exchanges)
+        float acc[G] = {};
+        for (int c0 = sub * VB;;) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int c = c0 + i * L * VB;
+#pragma unroll
+                for (int e = 0; e < VB; ++e)
+                    if (c + e < r)
+#pragma unroll
+                        for (int g = 0; g < G; ++g) acc[g] = fmaf(to_f32(wb[i].v[e]), us[(c + e) * G + g], acc[g]);
+            }
+            c0 += kAhead * L * VB;
+            if (c0 - sub * VB >= r) break;
+            ask(c0);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            for (int o = L / 2; o > 0; o /= 2) acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], o);
+            if (col[g] >= 0 && n < n1 && sub == (g & (L - 1))) t.dst[col[g] * t.sdst + n] = base[g] + acc[g];
+        }
+        n += rows;
+        if (nb + rows < n1) {
+            ask(sub * VB);
+            ask_base();
+        }
+    }
+    // no CTA leaves while another may still read its part
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <typename T, int VA, int VB, int NC>
+__global__ void __launch_bounds__(kThreads, LORA_MB) k_lora_cluster(const __grid_constant__ LoraParams P) {
     extern __shared__ __align__(16) float smem[];
-    __shared__ int cols[kGroup];
-    __shared__ int found;
     cg::cluster_group cluster = cg::this_cluster();
-    const int nc = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
     const LoraTask &t = P.task[blockIdx.y];
-    const int j = blockIdx.x / nc;
+    const int j = blockIdx.x / NC;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int a = slot_of(t, P.ids[j]);
+    // the columns that have this column's adapter, as a mask
+    const int id0 = lane < P.ncols ? P.ids[lane] : -1, id1 = lane + 32 < P.ncols ? P.ids[lane + 32] : -1;
+    const int a = slot_of(t, __shfl_sync(0xffffffffu, j < 32 ? id0 : id1, j & 31));
     const int r = a < 0 ? 0 : rank_of(t, a);
     if (r == 0) {  // nothing to add: the column's rows are base's
-        const int nper = (t.nrows + nc - 1) / nc;
+        const int me = static_cast<int>(cluster.block_rank());
+        const int nper = (t.nrows + NC - 1) / NC;
         const int n0 = min(t.nrows, me * nper), n1 = min(t.nrows, n0 + nper);
         for (int n = n0 + tid; n < n1; n += kThreads)
             t.dst[j * t.sdst + n] = t.base != nullptr ? t.base[j * t.sbase + n] : 0.0f;
         return;  // (the whole cluster takes this way)
     }
-    if (tid < 32) {
-        int before = 0;
-        for (int i = lane; i < j; i += 32) before += slot_of(t, P.ids[i]) == a;
-        before = __reduce_add_sync(0xffffffffu, before);
-        int n = 0;
-        if (before % kGroup == 0) {
-            for (int i0 = j; i0 < P.ncols && n < kGroup; i0 += 32) {
-                const unsigned m = __ballot_sync(0xffffffffu, i0 + lane < P.ncols && P.ids[min(i0 + lane, P.ncols - 1)] == a);
-                const int at = n + __popc(m & ((1u << lane) - 1));
-                if (((m >> lane) & 1u) && at < kGroup) cols[at] = i0 + lane;
-                n = min(kGroup, n + __popc(m));
-            }
-        }
-        if (lane == 0) found = n;
-    }
-    __syncthreads();
-    const int count = found;
-    if (count == 0) return;  // another column's cluster does this one (all CTAs agree)
+    uint64_t mask = __ballot_sync(0xffffffffu, id0 == a) | static_cast<uint64_t>(__ballot_sync(0xffffffffu, id1 == a)) << 32;
+    const uint64_t before = mask & ((uint64_t(1) << j) - 1);
+    if (__popcll(before) % kGroup != 0) return;  // another column's cluster does this one (all CTAs agree)
+    mask &= ~before;
     float *xs = smem, *part = smem + kGroup * kTile, *us = part + kGroup * t.rank;
+    const int count = __popcll(mask);
     if (count == 1)
-        lora_group<T, VA, VB, 1>(t, a, r, count, cols, xs, part, us, cluster);
+        lora_group<T, VA, VB, 1, NC>(t, a, r, mask, xs, part, us, cluster);
     else if (count <= 4)
-        lora_group<T, VA, VB, 4>(t, a, r, count, cols, xs, part, us, cluster);
+        lora_group<T, VA, VB, 4, NC>(t, a, r, mask, xs, part, us, cluster);
     else
-        lora_group<T, VA, VB, kGroup>(t, a, r, count, cols, xs, part, us, cluster);
+        lora_group<T, VA, VB, kGroup, NC>(t, a, r, mask, xs, part, us, cluster);
 }
 
 size_t cluster_smem(int rank) { return (kGroup * kTile + 2 * kGroup * rank) * sizeof(float); }
 
-template <typename T, int VA, int VB>
-cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
-    auto *fn = k_lora_cluster<T, VA, VB>;
+template <typename T, int VA, int VB, int NC>
+cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
+    auto *fn = k_lora_cluster<T, VA, VB, NC>;
     static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -303,20 +345,29 @@ cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    const int nc = 16;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.ncols * nc, ntasks);
+    cfg.gridDim = dim3(p.ncols * NC, ntasks);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = cluster_smem(rank);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = nc;
+    attr[0].val.clusterDim.x = NC;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+template <typename T, int VA, int VB>
+cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
+#ifdef LORA_NC
+    return launch_cluster_of<T, VA, VB, LORA_NC>(p, ntasks, rank, s);
+#else
+    return p.ncols * ntasks <= 18 ? launch_cluster_of<T, VA, VB, 16>(p, ntasks, rank, s)
+                                  : launch_cluster_of<T, VA, VB, 8>(p, ntasks, rank, s);
+#endif
 }
 
 // Whether chunks of V values of every row are 16-byte aligned.
