@@ -104,7 +104,10 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
 constexpr int kThreads = LORA_T;
 constexpr int kWarps = kThreads / 32;
 constexpr int kClusterCols = 64;  // columns up to which this kernel runs (bits of a mask)
-constexpr int kGroup = 8;         // columns of one adapter per cluster
+#ifndef LORA_G
+#define LORA_G 8
+#endif
+constexpr int kGroup = LORA_G;         // columns of one adapter per cluster
 constexpr int kTile = 1024;       // values of x per column in shared memory at a time
 constexpr int kBatch = 2;         // rows of A per warp and pass
 constexpr int kAhead = 4;         // chunks of a row of B in flight per lane
