@@ -5,8 +5,10 @@
 
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cstddef>
 
 using namespace q4k;
 namespace cg = cooperative_groups;
@@ -28,6 +30,7 @@ struct LogitsParams {
     int32_t *token;
     float *lse;
     int nvocab, max_history, n_bias, n_masks;
+    int slots;  // listed tokens a CTA has room for
 };
 
 #ifndef LG_NC
@@ -39,8 +42,10 @@ struct LogitsParams {
 #define LG_MB 4
 #endif
 constexpr int kThreads = LG_T;
-constexpr int kQuads = LG_Q;                      // groups of 4 tokens per thread and chunk
-constexpr int kChunk = kThreads * kQuads * 4;     // tokens whose counts and bias sums are in shared memory at a time
+constexpr int kQuads = LG_Q;                      // groups of 4 tokens per thread and chunk (at most 8)
+constexpr int kChunk = kThreads * kQuads * 4;     // tokens in flight per CTA
+constexpr int kSegment = 65536;                   // tokens whose listed places are held at a time
+constexpr int kMinSlots = 256, kMaxSlots = 4096;  // listed tokens with room for their count and bias sum
 constexpr int kAhead = 4;                         // list entries per thread in registers
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -69,62 +74,34 @@ __device__ __forceinline__ Stat shfl_xor(const Stat &v, int o) {
             __shfl_xor_sync(0xffffffffu, v.at, o)};
 }
 
-// Counts and bias sums of the listed tokens of one chunk. `touched` says which
-// places hold something; the others are zero throughout.
+// The listed tokens of one segment of a CTA's slice: a bit per token, the
+// number of bits before each word, and a slot {token, count, bias sum} per
+// listed token, found by its rank among them.
 struct Lists {
-    int count[kChunk];
-    float bias[kChunk];
-    uint32_t touched[kChunk / 32];
+    uint32_t touched[kSegment / 32];
+    uint16_t before[kSegment / 32];
+    uint32_t sums[kThreads / 32];
+    int token[kMaxSlots];  // `slots` of them, then as many counts and bias sums: the launch sizes the memory
 };
 
-// One warp adds 32 bias entries (lane order = list order) to the sums of the
-// chunk [base, base + n); entries outside it are left out.
-__device__ __forceinline__ void add_bias(Lists &S, int tok, float val, int base, int n, int lane) {
-    const bool in = tok >= 0 && tok >= base && tok - base < n;
-    if (!__any_sync(0xffffffffu, in)) return;
-    const int i = in ? tok - base : 0;
-    const unsigned same = __match_any_sync(0xffffffffu, in ? i : -1 - lane);
-    if (in) atomicOr(&S.touched[i >> 5], 1u << (i & 31));
-    if (__any_sync(0xffffffffu, __popc(same) > 1)) {
-        for (int q = 0; q < 32; ++q) {  // a token twice: one entry after the other
-            if (lane == q && in) S.bias[i] += val;
-            __syncwarp();
-        }
-    } else if (in) {
-        S.bias[i] += val;
-    }
-    __syncwarp();
-}
-
-__device__ __forceinline__ void add_count(Lists &S, int tok, int base, int n) {
-    if (tok >= 0 && tok >= base && tok - base < n) {
-        const int i = tok - base;
-        atomicOr(&S.touched[i >> 5], 1u << (i & 31));
-        atomicAdd(&S.count[i], 1);
-    }
-}
-
-// What a CTA knows of its column.
+// What a CTA knows of its column's lists: history entries [0, nh), bias entries
+// [b0, b1), the first of them in registers.
 struct Column {
-    const float *l;
-    float *d;
-    const uint32_t *mask;  // or NULL
     const int32_t *history;
-    int nh, b0, b1;        // history entries; bias entries [b0, b1)
-    float rep, freq, pres;
-    int v1;                // end of the CTA's tokens
-    int htok[kAhead], btok[kAhead];  // the lists' first entries
+    int nh, b0, b1;
+    int htok[kAhead], btok[kAhead];
     float bval[kAhead];
 };
 
-// Counts and bias sums of the chunk [base, base + n) from the column's lists.
-__device__ __forceinline__ void scan_lists(const LogitsParams &P, const Column &C, Lists &S, int base, int n) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // the bias entries go to the last warp, which has the fewest history entries
-    if (warp == kThreads / 32 - 1) {
+// f(token) for every history entry, by all threads; g(token, value, entries) for
+// the bias entries by the last warp, 32 entries in list order at a time.
+template <typename F, typename G>
+__device__ __forceinline__ void for_lists(const LogitsParams &P, const Column &C, F f, G g) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid / 32 == kThreads / 32 - 1) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-            if (C.b0 + i * 32 < C.b1) add_bias(S, C.btok[i], C.bval[i], base, n, lane);
+            if (C.b0 + i * 32 < C.b1) g(C.btok[i], C.bval[i]);
         for (int e0 = C.b0 + kAhead * 32; e0 < C.b1; e0 += kAhead * 32) {
             int tok[kAhead];
             float val[kAhead];
@@ -134,217 +111,293 @@ __device__ __forceinline__ void scan_lists(const LogitsParams &P, const Column &
                 tok[i] = e < C.b1 ? P.bias_tokens[e] : -1;
                 val[i] = e < C.b1 ? P.bias_values[e] : 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) add_bias(S, tok[i], val[i], base, n, lane);
+#pragma unroll 1
+            for (int i = 0; i < kAhead; ++i) g(tok[i], val[i]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add_count(S, C.htok[i], base, n);
+    for (int i = 0; i < kAhead; ++i) f(C.htok[i]);
     for (int e0 = kAhead * kThreads + tid; e0 < C.nh; e0 += kAhead * kThreads) {
         int tok[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) tok[i] = e0 + i * kThreads < C.nh ? C.history[e0 + i * kThreads] : -1;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) add_count(S, tok[i], base, n);
+        for (int i = 0; i < kAhead; ++i) f(tok[i]);
     }
 }
 
-// One chunk of tokens from `base` on. FULL: all kChunk tokens are the CTA's
-// and quads are aligned (V4); otherwise tokens outside [0, v1) are left out one by one.
-template <bool V4, bool FULL, bool MASKED>
-__device__ __forceinline__ void chunk(const LogitsParams &P, const Column &C, Lists &S, bool lists, bool stats, int base,
-                                      Stat &st) {
-    const int tid = threadIdx.x;
-    const int n = FULL ? kChunk : min(kChunk, C.v1 - base);
-    float z[kQuads][4];
-    uint32_t bits[kQuads];  // allowed tokens of the quad
-#pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-        const int v = base + (q * kThreads + tid) * 4;
-        uint32_t m = 15u;
-        if (MASKED) {
-            const int words = (P.nvocab + 31) / 32, lo = FULL ? v >> 5 : max(v, 0) >> 5;
-            const uint32_t w0 = FULL || lo < words ? C.mask[lo] : 0u;
-            const uint32_t w1 = lo + 1 < words && (v & 31) > 28 ? C.mask[lo + 1] : 0u;
-            m = FULL || v >= 0 ? __funnelshift_r(w0, w1, v & 31) & 15u : (w0 << -v) & 15u;
-        }
-        if (!FULL)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (v + e < 0 || v + e >= C.v1) m &= ~(1u << e);
-        bits[q] = m;
+// Finds the listed ones of the tokens [base, base + n): counts (integer
+// atomics: any order gives the same) and bias sums (one warp, in list order).
+// Returns how many there are; with more than `slots` nothing is summed.
+__device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C, Lists &S, int base, int n) {
+    const int tid = threadIdx.x, lane = tid & 31, words = (n + 31) / 32, slots = P.slots;
+    int *count = S.token + slots;
+    float *bias = reinterpret_cast<float *>(count + slots);
+    for (int i = tid; i < words; i += kThreads) S.touched[i] = 0u;
+    for (int i = tid; i < slots; i += kThreads) {
+        count[i] = 0;
+        bias[i] = 0.0f;
     }
-    // a logit is read where a token of its quad is allowed
+    __syncthreads();
+    auto in = [&](int tok) { return tok >= 0 && tok >= base && tok - base < n; };
+    auto mark = [&](int tok) {
+        if (in(tok)) atomicOr(&S.touched[(tok - base) >> 5], 1u << ((tok - base) & 31));
+    };
+    for_lists(P, C, mark, [&](int tok, float) { mark(tok); });
+    __syncthreads();
+    // a thread ranks a run of words
+    const int run = (words + kThreads - 1) / kThreads, w0 = tid * run, w1 = min(words, w0 + run);
+    uint32_t mine = 0;
+    for (int w = w0; w < w1; ++w) mine += __popc(S.touched[w]);
+    uint32_t upto = mine;
 #pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-        const int v = base + (q * kThreads + tid) * 4;
-        if (V4 && (FULL || (v >= 0 && v + 4 <= C.v1))) {
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (!MASKED || bits[q]) x = __ldcs(reinterpret_cast<const float4 *>(C.l + v));
-            z[q][0] = x.x, z[q][1] = x.y, z[q][2] = x.z, z[q][3] = x.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[q][e] = (bits[q] >> e) & 1u ? C.l[v + e] : 0.0f;
-        }
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
     }
-    if (lists) {
-        __syncthreads();  // the last chunk's places are zero again
-        scan_lists(P, C, S, base, n);
-        __syncthreads();
+    if (lane == 31) S.sums[tid / 32] = upto;
+    __syncthreads();
+    uint32_t total = 0, at = upto - mine;
 #pragma unroll
-        for (int q = 0; q < kQuads; ++q) {
-            const int i = (q * kThreads + tid) * 4;
-            const uint32_t hit = S.touched[i >> 5] >> (i & 31) & 15u;
-            if (hit) {
-                const float4 b = *reinterpret_cast<const float4 *>(S.bias + i);
-                const int4 c = *reinterpret_cast<const int4 *>(S.count + i);
-                const float bv[4] = {b.x, b.y, b.z, b.w};
-                const int cv[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[q][e] = __fadd_rn(z[q][e], bv[e]);
-                    if (cv[e] > 0) {
-                        float y = z[q][e];
-                        y = y > 0.0f ? __fdiv_rn(y, C.rep) : __fmul_rn(y, C.rep);
-                        z[q][e] = __fsub_rn(y, __fadd_rn(__fmul_rn(static_cast<float>(cv[e]), C.freq), C.pres));
-                    }
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < tid / 32) at += S.sums[w];
+        total += S.sums[w];
+    }
+    for (int w = w0; w < w1; ++w) {
+        S.before[w] = static_cast<uint16_t>(at);
+        at += __popc(S.touched[w]);
+    }
+    __syncthreads();
+    if (static_cast<int>(total) > slots) return static_cast<int>(total);
+    auto slot = [&](int tok) {
+        if (!in(tok)) return -1;
+        const int i = tok - base, k = S.before[i >> 5] + __popc(S.touched[i >> 5] & ((1u << (i & 31)) - 1u));
+        S.token[k] = tok;
+        return k;
+    };
+    for_lists(
+        P, C,
+        [&](int tok) {
+            const int i = slot(tok);
+            if (i >= 0) atomicAdd(&count[i], 1);
+        },
+        [&](int tok, float val) {
+            const int i = slot(tok);
+            if (!__any_sync(0xffffffffu, i >= 0)) return;
+            const unsigned same = __match_any_sync(0xffffffffu, i >= 0 ? i : -1 - lane);
+            if (__any_sync(0xffffffffu, __popc(same) > 1)) {
+                for (int q = 0; q < 32; ++q) {  // a token twice: one entry after the other
+                    if (lane == q && i >= 0) bias[i] += val;
+                    __syncwarp();
                 }
-                *reinterpret_cast<float4 *>(S.bias + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                *reinterpret_cast<int4 *>(S.count + i) = make_int4(0, 0, 0, 0);
-                atomicAnd(&S.touched[i >> 5], ~(15u << (i & 31)));
+            } else if (i >= 0) {
+                bias[i] += val;
             }
-        }
-    }
-    float m = st.m, top[kQuads];
-#pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-        const int v = base + (q * kThreads + tid) * 4;
-        if (MASKED || !FULL)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!((bits[q] >> e) & 1u)) z[q][e] = -INFINITY;
-        if (V4 && (FULL || (v >= 0 && v + 4 <= C.v1))) {
-            *reinterpret_cast<float4 *>(C.d + v) = make_float4(z[q][0], z[q][1], z[q][2], z[q][3]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (v + e >= 0 && v + e < C.v1) C.d[v + e] = z[q][e];
-        }
-        top[q] = fmaxf(fmaxf(z[q][0], z[q][1]), fmaxf(z[q][2], z[q][3]));  // (of numbers: NaN loses)
-        m = fmaxf(m, top[q]);
-    }
-    if (!stats) return;
-    // the chunk's maximum and its lowest quad (a thread's quads ascend), one rescaling of the sum, then the
-    // exponentials. -inf adds nothing even while it is all that has been seen; NaN stays in the sum.
-    if (m > st.m) {
-#pragma unroll
-        for (int q = kQuads - 1; q >= 0; --q)
-            if (top[q] == m) st.at = base + (q * kThreads + tid) * 4;
-        st.s *= ex2((st.m - m) * kLog2e);
-        st.m = m;
-    }
-    if (m == INFINITY) {
-#pragma unroll
-        for (int q = 0; q < kQuads; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st.s += z[q][e] == m ? 1.0f : z[q][e] != z[q][e] ? z[q][e] : 0.0f;
-        return;
-    }
-    // (the difference first: m log2(e) alone would overflow for the largest values)
-    const float around = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int q = 0; q < kQuads; ++q)
-        st.s += (ex2((z[q][0] - around) * kLog2e) + ex2((z[q][1] - around) * kLog2e)) +
-                (ex2((z[q][2] - around) * kLog2e) + ex2((z[q][3] - around) * kLog2e));
+            __syncwarp();
+        });
+    __syncthreads();
+    return static_cast<int>(total);
 }
 
-// A cluster per column; its CTAs split the vocabulary and walk their slices in
-// chunks of kChunk tokens. Per chunk: the logits are asked for; the column's
-// lists are scanned for tokens of the chunk, whose counts (integer atomics: any
-// order gives the same) and bias sums (one warp, in list order) meet in shared
-// memory; then every logit is finished in registers, stored, and taken into the
-// running statistics. The logits cross memory once in each direction.
+// The ends of a row, token by token: values of the tokens of [0, v1) at v..v+3.
+__device__ __forceinline__ float4 load_each(const float *l, int v, int v1) {
+    return make_float4(v >= 0 && v < v1 ? l[v] : -INFINITY, v + 1 >= 0 && v + 1 < v1 ? l[v + 1] : -INFINITY,
+                       v + 2 >= 0 && v + 2 < v1 ? l[v + 2] : -INFINITY, v + 3 >= 0 && v + 3 < v1 ? l[v + 3] : -INFINITY);
+}
+__device__ __noinline__ float4 load_end(const float *l, int v, int v1) { return load_each(l, v, v1); }
+// Stores those tokens of z whose bit is set.
+__device__ __forceinline__ void store_each(float *d, int v, float4 z, uint32_t bits) {
+    if (bits & 1u) d[v] = z.x;
+    if (bits & 2u) d[v + 1] = z.y;
+    if (bits & 4u) d[v + 2] = z.z;
+    if (bits & 8u) d[v + 3] = z.w;
+}
+// The bits of the tokens v..v+3 that lie in [0, v1).
+__device__ __forceinline__ uint32_t of_row(int v, int v1) {
+    return (v >= 0 ? 15u : 15u << -v) & (v + 4 <= v1 ? 15u : 15u >> (v + 4 - v1)) & 15u;
+}
+
+// A cluster per column; its CTAs split the vocabulary. A CTA first finds the
+// listed tokens of its slice (segments of 65536 tokens: a bitmap, ranks, a
+// slot per listed token), while its first logits are on their way; then a
+// thread per slot finishes the listed tokens, and the warps stream all others
+// without another barrier: kQuads loads of 16 bytes in flight per thread, every
+// logit stored and taken into the statistics. (Finishing listed tokens inside
+// the stream made every fourth quad of a warp wait for their chain of lookups.)
+// The logits cross memory once in each direction, and those of quads that a
+// mask forbids are not read. The CTAs' statistics meet in the
+// first one's shared memory; the others leave without waiting.
 // V4: rows of logits and dst are equally far from 16-byte boundaries, so four
-// tokens go in one access; chunks start on such a boundary (`shift` tokens
-// before a multiple of 4), the ends of a row are handled one by one.
+// tokens go in one access; quads start on such a boundary (`shift` tokens
+// before a multiple of 4), and only the quads at a row's ends go one by one.
 template <bool V4>
 __global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constant__ LogitsParams P) {
     extern __shared__ __align__(16) uint8_t smem[];
     Lists &S = *reinterpret_cast<Lists *>(smem);
-    __shared__ Stat part[kThreads / 32];
+    __shared__ Stat part[kThreads / 32], all[16];
     cg::cluster_group cluster = cg::this_cluster();
     const int nc = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
     const int64_t j = blockIdx.x / nc;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    Column C;
-    C.l = P.logits + j * P.s_col;
-    C.d = P.dst + j * P.s_dst;
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // (waited for below: every CTA has begun)
+    const float *l = P.logits + j * P.s_col;
+    float *d = P.dst + j * P.s_dst;
     // this CTA's tokens [v0, v1): whole quads of the row's alignment
-    const int shift = V4 ? static_cast<int>(reinterpret_cast<uintptr_t>(C.l) / 4 % 4) : 0;
+    const int shift = V4 ? static_cast<int>(reinterpret_cast<uintptr_t>(l) / 4 % 4) : 0;
     const int quads = (P.nvocab + shift + 3) / 4, per = (quads + nc - 1) / nc;
-    const int v0 = min(quads, me * per) * 4 - shift;
-    C.v1 = min(P.nvocab, min(quads, me * per + per) * 4 - shift);
-    C.nh = C.b0 = C.b1 = 0;
-    C.rep = 1.0f;
-    C.freq = C.pres = 0.0f;
-    C.mask = nullptr;
-    C.history = nullptr;
+    const int v0 = min(quads, me * per) * 4 - shift, v1 = min(P.nvocab, min(quads, me * per + per) * 4 - shift);
+    const uint32_t *mask = nullptr;
+    if (P.mask != nullptr) {
+        const int64_t r = P.mask_rows != nullptr ? P.mask_rows[j] : j;
+        if (r >= 0 && r < P.n_masks) mask = P.mask + r * P.s_mask;
+    }
+    Column C = {};
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (P.history != nullptr) {
         C.history = P.history + j * P.s_hist;
         C.nh = P.history_len != nullptr ? min(max(P.history_len[j], 0), P.max_history) : P.max_history;
-        C.rep = P.penalties[3 * j];
-        C.freq = P.penalties[3 * j + 1];
-        C.pres = P.penalties[3 * j + 2];
+        rep = P.penalties[3 * j];
+        freq = P.penalties[3 * j + 1];
+        pres = P.penalties[3 * j + 2];
     }
     if (P.bias_tokens != nullptr) {
         C.b0 = min(max(P.bias_offsets[j], 0), P.n_bias);
         C.b1 = min(max(P.bias_offsets[j + 1], C.b0), P.n_bias);
     }
-    if (P.mask != nullptr) {
-        const int64_t r = P.mask_rows != nullptr ? P.mask_rows[j] : j;
-        if (r >= 0 && r < P.n_masks) C.mask = P.mask + r * P.s_mask;
-    }
     const bool lists = C.nh > 0 || C.b1 > C.b0, stats = P.token != nullptr || P.lse != nullptr;
-    if (lists) {
-        for (int i = tid; i < static_cast<int>(sizeof(Lists) / 16); i += kThreads)
-            reinterpret_cast<int4 *>(&S)[i] = make_int4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            C.htok[i] = tid + i * kThreads < C.nh ? C.history[tid + i * kThreads] : -1;
-            const int e = C.b0 + lane + i * 32;
-            const bool mine = warp == kThreads / 32 - 1 && e < C.b1;
-            C.btok[i] = mine ? P.bias_tokens[e] : -1;
-            C.bval[i] = mine ? P.bias_values[e] : 0.0f;
-        }
+    for (int i = 0; i < kAhead; ++i) {
+        C.htok[i] = tid + i * kThreads < C.nh ? C.history[tid + i * kThreads] : -1;
+        const int e = C.b0 + lane + i * 32;
+        const bool mine = warp == kThreads / 32 - 1 && e < C.b1;
+        C.btok[i] = mine ? P.bias_tokens[e] : -1;
+        C.bval[i] = mine ? P.bias_values[e] : 0.0f;
     }
     Stat st = {-INFINITY, 0.0f, INT_MAX};
-    for (int base = v0; base < C.v1; base += kChunk) {
-        if (V4 && base >= 0 && base + kChunk <= C.v1) {
-            if (C.mask != nullptr)
-                chunk<V4, V4, true>(P, C, S, lists, stats, base, st);
+    float4 z[kQuads];
+    uint32_t allowed = ~0u;  // of the thread's quads, four bits each
+    // asks for the quads of [base, v1) that are the thread's
+    auto load = [&](int base) {
+        if (mask != nullptr) {
+            const int words = (P.nvocab + 31) / 32;
+            allowed = 0u;
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                const int v = base + (q * kThreads + tid) * 4, lo = max(v, 0) >> 5;
+                const uint32_t w0 = lo < words ? mask[lo] : 0u;
+                const uint32_t w1 = lo + 1 < words && (v & 31) > 28 ? mask[lo + 1] : 0u;
+                allowed |= ((v >= 0 ? __funnelshift_r(w0, w1, v & 31) : w0 << -v) & 15u) << (4 * q);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+            const int v = base + (q * kThreads + tid) * 4;
+            z[q] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (v >= v1 || !(allowed >> (4 * q) & 15u)) continue;
+            if (!V4)
+                z[q] = load_each(l, v, v1);
+            else if (v >= 0 && v + 4 <= v1)
+                z[q] = __ldcs(reinterpret_cast<const float4 *>(l + v));
             else
-                chunk<V4, V4, false>(P, C, S, lists, stats, base, st);
-        } else {
-            if (C.mask != nullptr)
-                chunk<V4, false, true>(P, C, S, lists, stats, base, st);
-            else
-                chunk<V4, false, false>(P, C, S, lists, stats, base, st);
+                z[q] = load_end(l, v, v1);
+        }
+    };
+    int seg = v0, room = kSegment;
+    if (v0 < v1) load(v0);
+    while (seg < v1) {
+        const int n = min(room, v1 - seg);
+        if (lists) {
+            const int total = scan_lists(P, C, S, seg, n);
+            if (total > P.slots) {  // more than there are slots for: segments of as many tokens
+                room = P.slots;
+                __syncthreads();
+                continue;
+            }
+            for (int i = tid; i < total; i += kThreads) {
+                const int v = S.token[i], c = S.token[P.slots + i];
+                float y = -INFINITY;
+                if (mask == nullptr || (mask[v >> 5] >> (v & 31) & 1u)) {
+                    y = __fadd_rn(l[v], __int_as_float(S.token[2 * P.slots + i]));
+                    if (c > 0) {
+                        y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                        y = __fsub_rn(y, __fadd_rn(__fmul_rn(static_cast<float>(c), freq), pres));
+                    }
+                }
+                d[v] = y;
+                // (NaN is never picked and stays in the sum)
+                take(st, {y == y ? y : -INFINITY, y == -INFINITY ? 0.0f : y == y ? 1.0f : y, v - (v - v0) % 4});
+            }
+        }
+        for (int base = seg; base < seg + n; base += kChunk) {
+            float m = st.m, top[kQuads];
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                const int i = base - seg + (q * kThreads + tid) * 4, v = seg + i;
+                top[q] = -INFINITY;
+                if (i >= n) continue;
+                const uint32_t ok = allowed >> (4 * q) & 15u, listed = lists ? S.touched[i >> 5] >> (i & 31) & 15u : 0u;
+                if (ok != 15u || listed != 0u) {
+                    const uint32_t out = ~ok | listed;
+                    if (out & 1u) z[q].x = -INFINITY;
+                    if (out & 2u) z[q].y = -INFINITY;
+                    if (out & 4u) z[q].z = -INFINITY;
+                    if (out & 8u) z[q].w = -INFINITY;
+                }
+                if (V4 && v >= 0 && v + 4 <= v1 && listed == 0u)
+                    *reinterpret_cast<float4 *>(d + v) = z[q];
+                else
+                    store_each(d, v, z[q], of_row(v, v1) & ~listed);
+                top[q] = fmaxf(fmaxf(z[q].x, z[q].y), fmaxf(z[q].z, z[q].w));  // (of numbers: NaN loses)
+                m = fmaxf(m, top[q]);
+            }
+            if (stats) {
+                // the chunk's maximum and its lowest quad, one rescaling of the sum, then the exponentials. -inf adds
+                // nothing even while it is all that has been seen; NaN stays in the sum. The difference comes first:
+                // m log2(e) alone would overflow for the largest values.
+                if (m > st.m) st.at = INT_MAX;
+                if (m > -INFINITY)
+#pragma unroll
+                    for (int q = kQuads - 1; q >= 0; --q)
+                        if (top[q] == m) st.at = min(st.at, base + (q * kThreads + tid) * 4);
+                if (m > st.m) {
+                    st.s *= ex2((st.m - m) * kLog2e);
+                    st.m = m;
+                }
+                const float around = m == -INFINITY ? 0.0f : m;
+                const bool inf = m == INFINITY;
+                auto term = [&](float x) {
+                    return inf ? (x == INFINITY ? 1.0f : x != x ? x : 0.0f) : ex2((x - around) * kLog2e);
+                };
+#pragma unroll
+                for (int q = 0; q < kQuads; ++q)
+                    if (base - seg + (q * kThreads + tid) * 4 < n)
+                        st.s += (term(z[q].x) + term(z[q].y)) + (term(z[q].z) + term(z[q].w));
+            }
+            const int next = base + kChunk < seg + n ? base + kChunk : seg + n;
+            if (next < v1) load(next);
+        }
+        seg += n;
+        if (lists && seg < v1) __syncthreads();  // the lists of this segment are done with
+    }
+    if (stats) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) take(st, shfl_xor(st, o));
+        if (lane == 0) part[warp] = st;
+        __syncthreads();
+        if (warp == 0) {
+            st = lane < kThreads / 32 ? part[lane] : Stat{-INFINITY, 0.0f, INT_MAX};
+#pragma unroll
+            for (int o = kThreads / 64; o > 0; o >>= 1) take(st, shfl_xor(st, o));
         }
     }
-    if (!stats) return;  // (the whole cluster)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) take(st, shfl_xor(st, o));
-    if (lane == 0) part[warp] = st;
-    __syncthreads();
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (!stats) return;
+    if (tid == 0) *cluster.map_shared_rank(all + me, 0) = st;
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (me != 0) return;
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 0) {
-        st = lane < kThreads / 32 ? part[lane] : Stat{-INFINITY, 0.0f, INT_MAX};
-#pragma unroll
-        for (int o = kThreads / 64; o > 0; o >>= 1) take(st, shfl_xor(st, o));
-        if (lane == 0) part[0] = st;
-    }
-    cluster.sync();
-    if (me == 0 && warp == 0) {
-        st = lane < nc ? cluster.map_shared_rank(part, lane)[0] : Stat{-INFINITY, 0.0f, INT_MAX};
+        st = lane < nc ? all[lane] : Stat{-INFINITY, 0.0f, INT_MAX};
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) take(st, shfl_xor(st, o));
         if (lane == 0) {
@@ -354,15 +407,16 @@ __global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constan
 #pragma unroll
                     for (int e = 3; e >= 0; --e) {
                         const int v = st.at + e;
-                        if (v >= 0 && v < P.nvocab && __ldcg(C.d + v) == st.m) at = v;
+                        if (v >= 0 && v < P.nvocab && __ldcg(d + v) == st.m) at = v;
                     }
                 P.token[j] = at;
             }
             if (P.lse != nullptr) P.lse[j] = st.s == 0.0f ? -INFINITY : (st.m == -INFINITY ? 0.0f : st.m) + logf(st.s);
         }
     }
-    cluster.sync();  // no CTA leaves while another may still read its part
 }
+
+size_t list_bytes(int slots) { return offsetof(Lists, token) + static_cast<size_t>(slots) * 12; }
 
 cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     const bool v4 = p.nvocab >= 16 && reinterpret_cast<uintptr_t>(p.logits) / 4 % 4 == reinterpret_cast<uintptr_t>(p.dst) / 4 % 4 &&
@@ -376,17 +430,23 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
         for (auto *f : {k_logits<true>, k_logits<false>}) {
             e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Lists)));
+                e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(list_bytes(kMaxSlots)));
             if (e != cudaSuccess) return e;
         }
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
+    // two CTAs for every SM if the vocabulary has a chunk for each
     int nc = 1;
-    while (nc < 16 && nc * kChunk < p.nvocab && (LG_NC ? nc < LG_NC : nc * static_cast<int64_t>(ncols) < 4096)) nc *= 2;
+    while (nc < 16 && nc * kChunk < p.nvocab && (LG_NC ? nc < LG_NC : nc * static_cast<int64_t>(ncols) < 296)) nc *= 2;
+    // slots for a column's whole history and its likely biases (their number per column is known to the device
+    // alone); a CTA whose tokens need more takes them in smaller segments
+    const int64_t listed = p.max_history + (p.bias_tokens != nullptr ? 2 * static_cast<int64_t>(p.n_bias) / ncols + 64 : 0);
+    LogitsParams q = p;
+    q.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, std::max<int64_t>(kMinSlots, (listed + 31) / 32 * 32)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(ncols) * nc);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.history != nullptr || p.bias_tokens != nullptr ? sizeof(Lists) : 0;
+    cfg.dynamicSmemBytes = p.history != nullptr || p.bias_tokens != nullptr ? list_bytes(q.slots) : 0;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -395,7 +455,7 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, p);
+    return cudaLaunchKernelEx(&cfg, fn, q);
 }
 
 }  // namespace
