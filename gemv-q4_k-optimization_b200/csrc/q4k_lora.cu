@@ -3,12 +3,14 @@
 //
 //   u[j][t]   = scale_a * sum_k A_a[t][k] x[j][k]        (shrink)
 //   dst[j][n] = base[j][n] + sum_t B_a[n][t] u[j][t]     (expand), a = ids[j]
+#include "q4k_device.cuh"
 #include "q4k_request.h"
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 using namespace q4k;
@@ -27,12 +29,21 @@ struct LoraTask {
     int u_off;  // first value of this task in a column's u
 };
 
+// Columns of one adapter that are worked on together (many columns).
+struct LoraTile {
+    int slot, first, count;  // slot (-1: no adapter), first place in the sorted order, columns
+};
+
 struct LoraParams {
     LoraTask task[Q4K_MAX_TASKS];
     const int32_t *ids;
-    float *u;       // ncols x u_cols
-    int u_cols;
-    int ncols;
+    int ntasks, ncols;
+    // many columns only: workspace and splits
+    int *ntiles;
+    LoraTile *tiles;
+    int *order;   // columns sorted by adapter
+    float *u;     // splits x ncols x u_cols, in sorted order
+    int u_cols, splits, max_slots, rows_per_cta;
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -45,45 +56,6 @@ __device__ __forceinline__ int rank_of(const LoraTask &t, int a) {
     if (t.ranks == nullptr) return t.rank;
     const int r = t.ranks[a];
     return r < 0 ? 0 : r > t.rank ? t.rank : r;
-}
-
-// One warp per (column, t): blockIdx.x = column, blockIdx.y = task, 8 warps over t.
-template <typename T>
-__global__ void __launch_bounds__(256) k_lora_shrink(const __grid_constant__ LoraParams P) {
-    const LoraTask &t = P.task[blockIdx.y];
-    const int64_t j = blockIdx.x;
-    const int a = slot_of(t, P.ids[j]);
-    if (a < 0) return;
-    const int r = rank_of(t, a);
-    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
-    const int lane = threadIdx.x & 31;
-    const float *x = t.x + j * t.sx;
-    for (int q = threadIdx.x >> 5; q < r; q += 8) {
-        const T *row = static_cast<const T *>(t.A) + a * t.sa_slot + q * t.sa_row;
-        float s = 0.0f;
-        for (int k = lane; k < t.K; k += 32) s = fmaf(to_f32(row[k]), x[k], s);
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) P.u[j * P.u_cols + t.u_off + q] = s * scale;
-    }
-}
-
-// One thread per output: blockIdx.x = column, blockIdx.y = task, threads over rows.
-template <typename T>
-__global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ LoraParams P) {
-    const LoraTask &t = P.task[blockIdx.y];
-    const int64_t j = blockIdx.x;
-    const int a = slot_of(t, P.ids[j]);
-    const int r = a < 0 ? 0 : rank_of(t, a);
-    const float *u = P.u + j * P.u_cols + t.u_off;
-    for (int n = blockIdx.z * 256 + threadIdx.x; n < t.nrows; n += gridDim.z * 256) {
-        float s = 0.0f;
-        if (r > 0) {
-            const T *row = static_cast<const T *>(t.B) + a * t.sb_slot + n * t.sb_row;
-            for (int q = 0; q < r; ++q) s = fmaf(to_f32(row[q]), u[q], s);
-        }
-        const float b = t.base != nullptr ? t.base[j * t.sbase + n] : 0.0f;
-        t.dst[j * t.sdst + n] = b + s;
-    }
 }
 
 // ---- few columns: one cluster per adapter and group of columns -------------------
@@ -373,29 +345,448 @@ cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream
 #endif
 }
 
-// Whether chunks of V values of every row are 16-byte aligned.
+// ---- many columns: grouped products on the tensor cores ----------------------------
+// Three launches: the columns are sorted by adapter into tiles of up to 64
+// columns of one adapter; shrink computes u for a tile, K split over CTAs;
+// expand adds the parts of u, and streams base -> dst. What has to move is x,
+// base and dst once (A and B are small and stay in L2), so both products only
+// have to keep up with memory. fp32 FMAs would not (4.3 GFLOP at rank 64,
+// 4096 columns, 4096 x 4096: 60 us against 31 us of traffic); tf32 and plain
+// bf16 would lose digits. So every fp32 value is cut into three bf16 pieces
+// that add up to it exactly (8 bits each), an fp16 weight into two, and the
+// products of pieces down to 2^-16 of the largest are summed on bf16 MMAs
+// (3 for bf16 weights, 5 for fp16, 6 for fp32); what is left out is below an
+// fp32 rounding. The MMAs' own sums are cut off, not rounded, so they are
+// taken over into fp32 registers after at most 12 of them.
+constexpr int kTileCols = 64;  // columns per tile
+constexpr int kRanks = 64;     // ranks per shrink CTA
+constexpr int kStageK = 64;    // values of K per stage of A in shared memory
+constexpr int kRing = 3;
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The upper halves of two fp32 values, a's in the lower half: bf16 pieces cut off towards zero.
+__device__ __forceinline__ uint32_t upper(float a, float b) {
+    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ float rest(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+template <int N> __device__ __forceinline__ void pieces(float a, float b, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        p[i] = upper(a, b);
+        a = rest(a);
+        b = rest(b);
+    }
+}
+template <typename T> struct Weight;  // bf16 pieces of a weight
+template <> struct Weight<__nv_bfloat16> { static constexpr int kPieces = 1; };
+template <> struct Weight<__half> { static constexpr int kPieces = 2; };
+template <> struct Weight<float> { static constexpr int kPieces = 3; };
+
+// Eight consecutive weights as MMA operands: q[piece][i] holds weights 2i, 2i + 1.
+template <typename T> struct Eight {
+    T v[8];
+};
+template <typename T> __device__ __forceinline__ void weights(const Eight<T> &w, uint32_t (&q)[Weight<T>::kPieces][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (Weight<T>::kPieces == 1) {
+            q[0][i] = *reinterpret_cast<const uint32_t *>(&w.v[2 * i]);
+        } else {
+            uint32_t p[Weight<T>::kPieces];
+            pieces(to_f32(w.v[2 * i]), to_f32(w.v[2 * i + 1]), p);
+#pragma unroll
+            for (int k = 0; k < Weight<T>::kPieces; ++k) q[k][i] = p[k];
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ Eight<T> load_eight_smem(const T *p) {
+    Eight<T> w;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        reinterpret_cast<uint4 *>(&w)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return w;
+}
+// Values [0, n) at p (n may be 0 or less), the others zero. V: p is 16-byte aligned.
+template <typename T, bool V> __device__ __forceinline__ Eight<T> load_eight(const T *p, int n) {
+    Eight<T> w;
+    if (V && n >= 8) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+            reinterpret_cast<uint4 *>(&w)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w.v[e] = e < n ? p[e] : T(0.0f);
+    }
+    return w;
+}
+
+// Sorts the columns by adapter (bins: the slots, then "none") and lists the tiles.
+__global__ void __launch_bounds__(1024) k_lora_plan(const __grid_constant__ LoraParams P) {
+    __shared__ int bin[Q4K_MAX_LORA_SLOTS + 1], at[Q4K_MAX_LORA_SLOTS + 1], warps[2][32];
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, bins = P.max_slots + 1;
+    auto bin_of = [&](int j) {
+        const int id = P.ids[j];
+        return id >= 0 && id < P.max_slots ? id : P.max_slots;
+    };
+    // one addition per warp and bin
+    auto add = [&](int *counts, int j) {
+        const bool live = j < P.ncols;
+        const int b = live ? bin_of(j) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, b);
+        const int lead = __ffs(same) - 1;
+        int first = 0;
+        if (live && lane == lead) first = atomicAdd(&counts[b], __popc(same));
+        return __shfl_sync(0xffffffffu, first, lead) + __popc(same & ((1u << lane) - 1));
+    };
+    for (int i = tid; i < bins; i += 1024) bin[i] = 0;
+    __syncthreads();
+    for (int j0 = tid - lane; j0 < P.ncols; j0 += 1024) add(bin, j0 + lane);
+    __syncthreads();
+    // exclusive sums over the bins: columns and tiles before each (bins <= 1025: thread 0 takes the last one too)
+    int c[2] = {0, 0}, upto[2];
+    const int mine = tid < bins ? bin[tid] : 0;
+    c[0] = mine;
+    c[1] = (mine + kTileCols - 1) / kTileCols;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        upto[k] = c[k];
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto[k], o);
+            if (lane >= o) upto[k] += v;
+        }
+        if (lane == 31) warps[k][tid / 32] = upto[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        for (int w = 0; w < tid / 32; ++w) upto[k] += warps[k][w];
+    auto list = [&](int b, int cols, int first, int tile) {
+        at[b] = first;
+        for (int i = 0; i < cols; i += kTileCols)
+            P.tiles[tile++] = {b < P.max_slots ? b : -1, first + i, min(kTileCols, cols - i)};
+        if (b == bins - 1) *P.ntiles = tile;
+    };
+    if (tid < bins) list(tid, mine, upto[0] - c[0], upto[1] - c[1]);
+    if (tid == 1023 && bins == 1025) list(1024, bin[1024], upto[0], upto[1]);
+    __syncthreads();
+    for (int j0 = tid - lane; j0 < P.ncols; j0 += 1024) {
+        const int p = add(at, j0 + lane);
+        if (j0 + lane < P.ncols) P.order[p] = j0 + lane;
+    }
+}
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src), "r"(bytes)
+                 : "memory");
+}
+
+// Stage of A in shared memory: kRanks rows of kStageK values, as kStageK / 32
+// slabs of 32 (rows 32 * sizeof(T) apart: the eight rows and four eights of a
+// fragment load cover all banks).
+constexpr int kStageValues = kRanks * kStageK;
+
+// u of a tile's columns for kRanks ranks, over this CTA's share of K. Four
+// warps, 16 columns each: x goes from memory straight into MMA fragments
+// (lane t of a row takes eights of consecutive values; A is read in the same
+// order, so the sum is over the same pairs), A through shared memory.
+template <typename T, bool VX, bool VA>
+__global__ void __launch_bounds__(128) k_lora_shrink(const __grid_constant__ LoraParams P) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    T *stage = reinterpret_cast<T *>(smem_raw);
+    pdl_launch_dependents();
+    pdl_wait();
+    if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;
+    const LoraTile tile = P.tiles[blockIdx.x];
+    int z = blockIdx.z, ti = 0;
+    while (z >= (P.task[ti].rank + kRanks - 1) / kRanks) z -= (P.task[ti++].rank + kRanks - 1) / kRanks;
+    const LoraTask &t = P.task[ti];
+    const int a = slot_of(t, tile.slot), r = a < 0 ? 0 : rank_of(t, a), r0 = z * kRanks;
+    if (r0 >= r) return;
+    const int nr = min(kRanks, r - r0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, q = lane & 3;
+    // this CTA's share of K: whole stages
+    const int stages = (t.K + kStageK - 1) / kStageK, per = (stages + P.splits - 1) / P.splits;
+    const int s0 = min(stages, static_cast<int>(blockIdx.y) * per), s1 = min(stages, s0 + per);
+    const bool busy = warp * 16 < tile.count;
+    const float *xr[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = warp * 16 + g + 8 * h;
+        xr[h] = i < tile.count ? t.x + P.order[tile.first + i] * t.sx : nullptr;
+    }
+    const T *A = static_cast<const T *>(t.A) + a * t.sa_slot + r0 * t.sa_row;
+    auto fill = [&](int s) {
+        T *to = stage + (s % kRing) * kStageValues;
+        if (s < s1) {
+            if constexpr (VA) {
+                constexpr int E = 16 / sizeof(T), C = kStageK / E;  // values per copy, copies per row
+                for (int i = tid; i < kRanks * C; i += 128) {
+                    const int row = i / C, k = (i - row * C) * E, left = row < nr ? min(E, t.K - s * kStageK - k) : 0;
+                    const bool some = left > 0;
+                    cp_async16(to + ((k / 32) * kRanks + row) * 32 + k % 32, some ? A + row * t.sa_row + s * kStageK + k : A,
+                               some ? left * static_cast<int>(sizeof(T)) : 0);
+                }
+            } else {
+                for (int i = tid; i < kRanks * kStageK; i += 128) {
+                    const int row = i / kStageK, k = i % kStageK;
+                    to[((k / 32) * kRanks + row) * 32 + k % 32] =
+                        row < nr && s * kStageK + k < t.K ? A[row * t.sa_row + s * kStageK + k] : T(0.0f);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto load_x = [&](Eight<float> (&x)[2], int k) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[h] = load_eight<float, VX>(xr[h] + k + 8 * q, xr[h] != nullptr ? t.K - k - 8 * q : 0);
+    };
+    float sum[8][4] = {};
+    Eight<float> x[2];
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) fill(s0 + i);
+    if (busy && s0 < s1) load_x(x, s0 * kStageK);
+    for (int s = s0; s < s1; ++s) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        __syncthreads();  // stage s has come, and stage s - 1 may be written again
+        fill(s + kRing - 1);
+        if (!busy) continue;
+        const T *w = stage + (s % kRing) * kStageValues;
+#pragma unroll
+        for (int half = 0; half < kStageK / 32; ++half) {
+            uint32_t xa[2][3][4];  // [MMA][piece][operand registers]
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t p[3];
+                    pieces(x[h].v[2 * i], x[h].v[2 * i + 1], p);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) xa[i / 2][k][(i % 2) * 2 + h] = p[k];
+                }
+            const int k = s * kStageK + half * 32 + 32;
+            if (half == 0 || s + 1 < s1) load_x(x, k);  // (zeros behind K)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                if (n * 8 >= nr) break;
+                uint32_t wq[Weight<T>::kPieces][4];
+                weights(load_eight_smem(w + (half * kRanks + n * 8 + g) * 32 + 8 * q), wq);
+                float acc[4] = {};
+#pragma unroll
+                for (int i = 2; i >= 0; --i)
+#pragma unroll
+                    for (int k2 = Weight<T>::kPieces - 1; k2 >= 0; --k2)
+                        if (i + k2 <= 2)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) mma_bf16(acc, xa[m][i], wq[k2][2 * m], wq[k2][2 * m + 1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[n][e] += acc[e];
+            }
+        }
+    }
+    if (!busy) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = warp * 16 + g + 8 * h;
+        if (i >= tile.count) continue;
+        float *u = P.u + (static_cast<int64_t>(blockIdx.y) * P.ncols + tile.first + i) * P.u_cols + t.u_off + r0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (n * 8 + 2 * q + e < nr) u[n * 8 + 2 * q + e] = sum[n][2 * h + e];
+    }
+}
+
+// dst of a tile's columns for a range of rows. The pieces of u go to shared
+// memory once; then each warp walks blocks of 16 columns x 32 rows. The rows
+// of a block are dealt to the MMAs' columns so that a lane ends with eight
+// consecutive rows of two columns: base and dst move in 16-byte accesses.
+template <typename T, bool VB, bool VY>
+__global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ LoraParams P) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    pdl_launch_dependents();
+    pdl_wait();
+    if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;
+    const LoraTile tile = P.tiles[blockIdx.x];
+    const LoraTask &t = P.task[blockIdx.z];
+    const int n0 = blockIdx.y * P.rows_per_cta, n1 = min(t.nrows, n0 + P.rows_per_cta);
+    if (n0 >= n1) return;
+    const int a = slot_of(t, tile.slot), r = a < 0 ? 0 : rank_of(t, a);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    if (r == 0) {  // nothing to add
+        for (int i = warp; i < tile.count; i += 8) {
+            const int64_t j = P.order[tile.first + i];
+            for (int n = n0 + lane; n < n1; n += 32) t.dst[j * t.sdst + n] = t.base != nullptr ? t.base[j * t.sbase + n] : 0.0f;
+        }
+        return;
+    }
+    const int rp = (r + 31) / 32 * 32, pitch = rp + 8;  // (an odd number of 16-byte units: no bank twice)
+    uint16_t *up = reinterpret_cast<uint16_t *>(smem_raw);  // [piece][column][pitch]
+    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
+    for (int i = tid; i < tile.count * (rp / 2); i += 256) {
+        const int col = i / (rp / 2), k = (i - col * (rp / 2)) * 2;
+        float v[2] = {0.0f, 0.0f};
+        const float *u = P.u + (static_cast<int64_t>(tile.first) + col) * P.u_cols + t.u_off + k;
+        for (int s = 0; s < P.splits; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (k + e < r) v[e] += u[static_cast<int64_t>(s) * P.ncols * P.u_cols + e];
+        uint32_t p[3];
+        pieces(v[0] * scale, v[1] * scale, p);
+#pragma unroll
+        for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t *>(up + (e * kTileCols + col) * pitch + k) = p[e];
+    }
+    __syncthreads();
+    const int m0 = (warp & 3) * 16;
+    if (m0 >= tile.count) return;
+    int64_t col[2];
+    bool live[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        live[h] = m0 + g + 8 * h < tile.count;
+        col[h] = P.order[tile.first + (live[h] ? m0 + g + 8 * h : 0)];
+    }
+    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
+    for (int nb = n0 + (warp >> 2) * 32; nb < n1; nb += 64) {
+        // base first: it is what the block waits for
+        const int n = nb + 8 * q;
+        Eight<float> y[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) y[h] = load_eight<float, VY>(t.base + col[h] * t.sbase + n, t.base != nullptr && live[h] ? n1 - n : 0);
+        float sum[4][4] = {};
+        for (int k = 0; k < rp; k += 32) {
+            uint32_t ua[2][3][4];
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // (rows behind the tile's columns hold anything: an MMA keeps rows apart)
+                    const uint4 v = *reinterpret_cast<const uint4 *>(up + (e * kTileCols + m0 + g + 8 * h) * pitch + k + 8 * q);
+                    ua[0][e][h] = v.x, ua[0][e][2 + h] = v.y, ua[1][e][h] = v.z, ua[1][e][2 + h] = v.w;
+                }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int row = nb + 8 * (g >> 1) + 2 * b + (g & 1);
+                uint32_t wq[Weight<T>::kPieces][4];
+                weights(load_eight<T, VB>(B + row * t.sb_row + k + 8 * q, row < n1 ? r - k - 8 * q : 0), wq);
+                float acc[4] = {};
+#pragma unroll
+                for (int i = 2; i >= 0; --i)
+#pragma unroll
+                    for (int k2 = Weight<T>::kPieces - 1; k2 >= 0; --k2)
+                        if (i + k2 <= 2)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) mma_bf16(acc, ua[m][i], wq[k2][2 * m], wq[k2][2 * m + 1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[b][e] += acc[e];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!live[h]) continue;
+            float *d = t.dst + col[h] * t.sdst + n;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) y[h].v[2 * b + e] += sum[b][2 * h + e];
+            if (VY && n + 8 <= n1) {
+                reinterpret_cast<float4 *>(d)[0] = reinterpret_cast<float4 *>(&y[h])[0];
+                reinterpret_cast<float4 *>(d)[1] = reinterpret_cast<float4 *>(&y[h])[1];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < n1) d[e] = y[h].v[e];
+            }
+        }
+    }
+}
+
+size_t shrink_smem(int esz) { return static_cast<size_t>(kRing) * kRanks * kStageK * esz; }
+size_t expand_smem(int rank) { return static_cast<size_t>(3) * kTileCols * ((rank + 31) / 32 * 32 + 8) * 2; }
+
+// A launch that may begin while the one before it ends (its kernel waits for it).
+template <typename K>
+cudaError_t launch_next(K *fn, dim3 grid, int threads, size_t smem, const LoraParams &p, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+// Tiles there can be: whole ones, and one begun per bin.
+int most_tiles(int ncols, int max_slots) { return ncols / kTileCols + (ncols < max_slots + 1 ? ncols : max_slots + 1); }
+
+template <typename T>
+cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool vy, int rank, cudaStream_t s) {
+    auto *shrink = vx ? va ? k_lora_shrink<T, true, true> : k_lora_shrink<T, true, false>
+                      : va ? k_lora_shrink<T, false, true> : k_lora_shrink<T, false, false>;
+    auto *expand = vb ? vy ? k_lora_expand<T, true, true> : k_lora_expand<T, true, false>
+                      : vy ? k_lora_expand<T, false, true> : k_lora_expand<T, false, false>;
+    static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        const int ss = static_cast<int>(shrink_smem(sizeof(T))), es = static_cast<int>(expand_smem(Q4K_MAX_LORA_RANK));
+        for (auto *f : {k_lora_shrink<T, true, true>, k_lora_shrink<T, true, false>, k_lora_shrink<T, false, true>,
+                        k_lora_shrink<T, false, false>})
+            if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ss)) != cudaSuccess) return e;
+        for (auto *f : {k_lora_expand<T, true, true>, k_lora_expand<T, true, false>, k_lora_expand<T, false, true>,
+                        k_lora_expand<T, false, false>})
+            if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, es)) != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    }
+    const unsigned tiles = static_cast<unsigned>(most_tiles(p.ncols, p.max_slots));
+    k_lora_plan<<<1, 1024, 0, s>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    unsigned chunks = 0, rows = 0;
+    for (int i = 0; i < p.ntasks; ++i) {
+        chunks += (p.task[i].rank + kRanks - 1) / kRanks;
+        rows = std::max(rows, static_cast<unsigned>(p.task[i].nrows));
+    }
+    if (chunks > 0) {
+        e = launch_next(shrink, dim3(tiles, p.splits, chunks), 128, shrink_smem(sizeof(T)), p, s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 256, expand_smem(rank),
+                       p, s);
+}
+
+// Whether every run of 8 values of every row is 16-byte aligned.
 bool rows_aligned(const void *p, int64_t slot, int64_t row, int esz) {
     return aligned_to(p, 16) && slot * esz % 16 == 0 && row * esz % 16 == 0;
 }
 
-template <typename T>
-cudaError_t launch_lora(const LoraParams &p, int ntasks, cudaStream_t s) {
-    if (p.ncols <= kClusterCols) {
-        constexpr int V = 16 / sizeof(T);
-        bool va = true, vb = true;
-        int rank = 0;
-        for (int i = 0; i < ntasks; ++i) {
-            const LoraTask &t = p.task[i];
-            va = va && rows_aligned(t.A, t.sa_slot, t.sa_row, sizeof(T));
-            vb = vb && rows_aligned(t.B, t.sb_slot, t.sb_row, sizeof(T));
-            rank = t.rank > rank ? t.rank : rank;
-        }
-        return va ? vb ? launch_cluster<T, V, V>(p, ntasks, rank, s) : launch_cluster<T, V, 1>(p, ntasks, rank, s)
-                  : vb ? launch_cluster<T, 1, V>(p, ntasks, rank, s) : launch_cluster<T, 1, 1>(p, ntasks, rank, s);
+template <typename T> cudaError_t launch_lora(const LoraParams &p, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    bool va = true, vb = true, vx = true, vy = true;
+    int rank = 0;
+    for (int i = 0; i < p.ntasks; ++i) {
+        const LoraTask &t = p.task[i];
+        va = va && rows_aligned(t.A, t.sa_slot, t.sa_row, sizeof(T));
+        vb = vb && rows_aligned(t.B, t.sb_slot, t.sb_row, sizeof(T));
+        vx = vx && rows_aligned(t.x, 0, t.sx, 4);
+        vy = vy && rows_aligned(t.dst, 0, t.sdst, 4) && rows_aligned(t.base, 0, t.base != nullptr ? t.sbase : 0, 4);
+        rank = std::max(rank, t.rank);
     }
-    k_lora_shrink<T><<<dim3(p.ncols, ntasks), 256, 0, s>>>(p);
-    k_lora_expand<T><<<dim3(p.ncols, ntasks, 8), 256, 0, s>>>(p);
-    return cudaGetLastError();
+    if (p.ncols > kClusterCols) return launch_grouped<T>(p, vx, va, vb, vy, rank, s);
+    const int n = p.ntasks;
+    return va ? vb ? launch_cluster<T, V, V>(p, n, rank, s) : launch_cluster<T, V, 1>(p, n, rank, s)
+              : vb ? launch_cluster<T, 1, V>(p, n, rank, s) : launch_cluster<T, 1, 1>(p, n, rank, s);
 }
 
 int type_bytes(int type) { return type == Q4K_TYPE_F32 ? 4 : type == Q4K_TYPE_F16 || type == Q4K_TYPE_BF16 ? 2 : 0; }
@@ -475,12 +866,31 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
     return Q4K_OK;
 }
 
-size_t workspace_need(const q4k_lora_task *tasks, int ntasks, int ncols) {
-    if (ncols <= kClusterCols) return 0;
-    size_t u = 0;
-    for (int i = 0; i < ntasks; ++i)
-        if (tasks[i].nrows > 0) u += static_cast<size_t>(tasks[i].rank);
-    return u * static_cast<size_t>(ncols) * sizeof(float);
+// Workspace of the many-column path: number of tiles, tiles, order, u.
+struct LoraLayout {
+    size_t tiles = 0, order = 0, u = 0, total = 0;
+    int max_slots = 0, u_cols = 0, splits = 1;
+};
+
+LoraLayout lora_layout(const q4k_lora_task *tasks, int ntasks, int ncols) {
+    LoraLayout L;
+    if (ncols <= kClusterCols) return L;
+    int64_t K = 0;
+    for (int i = 0; i < ntasks; ++i) {
+        if (tasks[i].nrows == 0) continue;
+        L.max_slots = std::max(L.max_slots, tasks[i].slots);
+        L.u_cols += tasks[i].rank;
+        K = std::max(K, tasks[i].K);
+    }
+    // K is split until there are two or three CTAs for each of the SMs, but not below four stages
+    const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
+    while (L.splits < 16 && tiles * L.splits < 256 && K >= 2 * L.splits * 4 * kStageK) L.splits *= 2;
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    L.tiles = 256;
+    L.order = L.tiles + up(static_cast<size_t>(most_tiles(ncols, L.max_slots)) * sizeof(LoraTile));
+    L.u = L.order + up(static_cast<size_t>(ncols) * 4);
+    L.total = L.u + up(static_cast<size_t>(L.splits) * ncols * L.u_cols * 4);
+    return L;
 }
 
 }  // namespace
@@ -489,7 +899,7 @@ extern "C" {
 
 size_t q4k_lora_workspace_bytes(const q4k_lora_task *tasks, int ntasks, int ncols) {
     if (check_tasks(tasks, ntasks, ncols) != Q4K_OK) return 0;
-    return workspace_need(tasks, ntasks, ncols);
+    return lora_layout(tasks, ntasks, ncols).total;
 }
 
 int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int32_t *ids, void *workspace,
@@ -498,7 +908,8 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
     if (st != Q4K_OK) return st;
     if (ncols == 0 || ntasks == 0) return Q4K_OK;
     if (ids == nullptr || !aligned_to(ids, 4)) return request_fail(Q4K_EINVAL, "ids null or not 4-byte aligned");
-    const size_t need = workspace_need(tasks, ntasks, ncols);
+    const LoraLayout L = lora_layout(tasks, ntasks, ncols);
+    const size_t need = L.total;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256)))
         return request_fail(Q4K_EWORKSPACE, "workspace %p of %zu bytes; need %zu bytes, 256-byte aligned", workspace,
                             workspace_bytes, need);
@@ -516,12 +927,28 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
     }
     if (n == 0) return Q4K_OK;
     p.ids = ids;
-    p.u = static_cast<float *>(workspace);
     p.ncols = ncols;
+    p.ntasks = n;
+    if (ncols > kClusterCols) {
+        uint8_t *ws = static_cast<uint8_t *>(workspace);
+        p.ntiles = reinterpret_cast<int *>(ws);
+        p.tiles = reinterpret_cast<LoraTile *>(ws + L.tiles);
+        p.order = reinterpret_cast<int *>(ws + L.order);
+        p.u = reinterpret_cast<float *>(ws + L.u);
+        p.splits = L.splits;
+        p.max_slots = L.max_slots;
+        // rows per expand CTA: few enough for several CTAs per SM
+        int64_t rows = 0;
+        for (int i = 0; i < n; ++i) rows += p.task[i].nrows;
+        p.rows_per_cta = 512;
+        const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
+        while (p.rows_per_cta > 64 && tiles * (rows / p.rows_per_cta) < 592) p.rows_per_cta /= 2;
+        while (rows / p.rows_per_cta >= 65535) p.rows_per_cta *= 2;  // (a grid's second dimension)
+    }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const cudaError_t e = tasks[0].type == Q4K_TYPE_F32   ? launch_lora<float>(p, n, s)
-                          : tasks[0].type == Q4K_TYPE_F16 ? launch_lora<__half>(p, n, s)
-                                                          : launch_lora<__nv_bfloat16>(p, n, s);
+    const cudaError_t e = tasks[0].type == Q4K_TYPE_F32   ? launch_lora<float>(p, s)
+                          : tasks[0].type == Q4K_TYPE_F16 ? launch_lora<__half>(p, s)
+                                                          : launch_lora<__nv_bfloat16>(p, s);
     if (e != cudaSuccess) return request_cuda_fail(e, "lora launch");
     return Q4K_OK;
 }
