@@ -364,8 +364,7 @@ constexpr int kStageK = 64;    // values of K per stage of A in shared memory
 constexpr int kRing = 3;
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -423,6 +422,31 @@ template <typename T, bool V> __device__ __forceinline__ Eight<T> load_eight(con
         for (int e = 0; e < 8; ++e) w.v[e] = e < n ? p[e] : T(0.0f);
     }
     return w;
+}
+
+// acc = the products of 16 rows of fp32 pieces with 4 x 8 rows of weights over
+// 32 values each: weight(b) gives lane (g, q) its eight weights of row g of the
+// b-th eight. The small products come first; the four sums are independent, so
+// their MMAs follow one another without waiting.
+template <typename T, typename F>
+__device__ __forceinline__ void products(float (&acc)[4][4], const uint32_t (&a)[2][3][4], F weight) {
+    constexpr int N = Weight<T>::kPieces;
+    uint32_t wq[4][N][4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        weights(weight(b), wq[b]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[b][e] = 0.0f;
+    }
+#pragma unroll
+    for (int order = 2; order >= 0; --order)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k <= order)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) mma_bf16(acc[b], a[m][order - k], wq[b][k][2 * m], wq[b][k][2 * m + 1]);
 }
 
 // Sorts the columns by adapter (bins: the slots, then "none") and lists the tiles.
@@ -573,20 +597,14 @@ __global__ void __launch_bounds__(128) k_lora_shrink(const __grid_constant__ Lor
             const int k = s * kStageK + half * 32 + 32;
             if (half == 0 || s + 1 < s1) load_x(x, k);  // (zeros behind K)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
+            for (int n = 0; n < 8; n += 4) {
                 if (n * 8 >= nr) break;
-                uint32_t wq[Weight<T>::kPieces][4];
-                weights(load_eight_smem(w + (half * kRanks + n * 8 + g) * 32 + 8 * q), wq);
-                float acc[4] = {};
+                float acc[4][4];
+                products<T>(acc, xa, [&](int b) { return load_eight_smem(w + (half * kRanks + (n + b) * 8 + g) * 32 + 8 * q); });
 #pragma unroll
-                for (int i = 2; i >= 0; --i)
+                for (int b = 0; b < 4; ++b)
 #pragma unroll
-                    for (int k2 = Weight<T>::kPieces - 1; k2 >= 0; --k2)
-                        if (i + k2 <= 2)
-#pragma unroll
-                            for (int m = 0; m < 2; ++m) mma_bf16(acc, xa[m][i], wq[k2][2 * m], wq[k2][2 * m + 1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[n][e] += acc[e];
+                    for (int e = 0; e < 4; ++e) sum[n + b][e] += acc[b][e];
             }
         }
     }
@@ -604,13 +622,22 @@ __global__ void __launch_bounds__(128) k_lora_shrink(const __grid_constant__ Lor
     }
 }
 
-// dst of a tile's columns for a range of rows. The pieces of u go to shared
-// memory once; then each warp walks blocks of 16 columns x 32 rows. The rows
-// of a block are dealt to the MMAs' columns so that a lane ends with eight
-// consecutive rows of two columns: base and dst move in 16-byte accesses.
+// dst of a tile's columns for a range of rows. Eight warps: 16 columns each, two
+// row groups. The pieces of u lie in shared memory; B comes through a ring of
+// stages of 64 rows x 64 ranks (32 in fp32, to fit beside the u of 512 ranks),
+// read once per CTA. A block is 16 columns x 32 rows; its rows are dealt
+// to the MMAs' columns so that a lane ends with eight consecutive rows of two
+// columns: base (asked for one block ahead) and dst move in 16-byte accesses.
+template <typename T> struct RowStage {
+    static constexpr int kK = sizeof(T) == 2 ? 64 : 32;  // ranks
+    static constexpr int kPitch = kK + 8;                // values between rows (rows meet in few banks)
+    static constexpr int kValues = 64 * kPitch;
+};
+
 template <typename T, bool VB, bool VY>
-__global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ LoraParams P) {
+__global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ LoraParams P) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
+    constexpr int kK = RowStage<T>::kK, kPitch = RowStage<T>::kPitch, kValues = RowStage<T>::kValues;
     pdl_launch_dependents();
     pdl_wait();
     if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;
@@ -627,8 +654,54 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
         }
         return;
     }
-    const int rp = (r + 31) / 32 * 32, pitch = rp + 8;  // (an odd number of 16-byte units: no bank twice)
-    uint16_t *up = reinterpret_cast<uint16_t *>(smem_raw);  // [piece][column][pitch]
+    T *ring = reinterpret_cast<T *>(smem_raw);
+    const int chunks = (r + kK - 1) / kK, rp = chunks * kK, pitch = rp + 8;
+    uint16_t *up = reinterpret_cast<uint16_t *>(ring + kRing * kValues);  // [piece][column][pitch]
+    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
+    const int stages = (n1 - n0 + 63) / 64 * chunks;
+    auto fill = [&](int s) {
+        if (s < stages) {
+            T *to = ring + (s % kRing) * kValues;
+            const int k0 = s % chunks * kK, row0 = n0 + s / chunks * 64;
+            if constexpr (VB) {
+                constexpr int E = 16 / sizeof(T), C = kK / E;  // values per copy, copies per row
+#pragma unroll
+                for (int i = tid; i < 64 * C; i += 256) {
+                    const int row = i / C, k = (i - row * C) * E, left = row0 + row < n1 ? min(E, r - k0 - k) : 0;
+                    const bool some = left > 0;
+                    cp_async16(to + row * kPitch + k, some ? B + (row0 + row) * t.sb_row + k0 + k : B,
+                               some ? left * static_cast<int>(sizeof(T)) : 0);
+                }
+            } else {
+                for (int i = tid; i < 64 * kK; i += 256) {
+                    const int row = i / kK, k = i % kK;
+                    to[row * kPitch + k] = row0 + row < n1 && k0 + k < r ? B[(row0 + row) * t.sb_row + k0 + k] : T(0.0f);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) fill(i);
+
+    const int m0 = (warp & 3) * 16;
+    const bool busy = m0 < tile.count;
+    const float *base[2];
+    float *dst[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = m0 + g + 8 * h;
+        const int64_t j = i < tile.count ? P.order[tile.first + i] : -1;
+        base[h] = j >= 0 && t.base != nullptr ? t.base + j * t.sbase : nullptr;
+        dst[h] = j >= 0 ? t.dst + j * t.sdst : nullptr;
+    }
+    int n = n0 + (warp >> 2) * 32 + 8 * q;  // the lane's first row of the block
+    auto load_base = [&](Eight<float> (&y)[2], int row) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) y[h] = load_eight<float, VY>(base[h] + row, base[h] != nullptr ? n1 - row : 0);
+    };
+    Eight<float> y[2];
+    load_base(y, n);
     const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
     for (int i = tid; i < tile.count * (rp / 2); i += 256) {
         const int col = i / (rp / 2), k = (i - col * (rp / 2)) * 2;
@@ -643,59 +716,49 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
 #pragma unroll
         for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t *>(up + (e * kTileCols + col) * pitch + k) = p[e];
     }
-    __syncthreads();
-    const int m0 = (warp & 3) * 16;
-    if (m0 >= tile.count) return;
-    int64_t col[2];
-    bool live[2];
+    float sum[4][4] = {};
+    for (int s = 0, c = 0; s < stages; ++s, c = c + 1 == chunks ? 0 : c + 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        __syncthreads();  // stage s (and at first u) has come, and stage s - 1 may be written again
+        fill(s + kRing - 1);
+        if (!busy) continue;
+        const T *w = ring + (s % kRing) * kValues + (warp >> 2) * 32 * kPitch;
+        Eight<float> next[2];
+        if (c + 1 == chunks) load_base(next, n + 64);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        live[h] = m0 + g + 8 * h < tile.count;
-        col[h] = P.order[tile.first + (live[h] ? m0 + g + 8 * h : 0)];
-    }
-    const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
-    for (int nb = n0 + (warp >> 2) * 32; nb < n1; nb += 64) {
-        // base first: it is what the block waits for
-        const int n = nb + 8 * q;
-        Eight<float> y[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) y[h] = load_eight<float, VY>(t.base + col[h] * t.sbase + n, t.base != nullptr && live[h] ? n1 - n : 0);
-        float sum[4][4] = {};
-        for (int k = 0; k < rp; k += 32) {
+        for (int k = 0; k < kK / 32; ++k) {
+            if (c * kK + k * 32 >= r) break;
             uint32_t ua[2][3][4];
 #pragma unroll
-            for (int e = 0; e < 3; ++e)
+            for (int i = 0; i < 3; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // (rows behind the tile's columns hold anything: an MMA keeps rows apart)
-                    const uint4 v = *reinterpret_cast<const uint4 *>(up + (e * kTileCols + m0 + g + 8 * h) * pitch + k + 8 * q);
-                    ua[0][e][h] = v.x, ua[0][e][2 + h] = v.y, ua[1][e][h] = v.z, ua[1][e][2 + h] = v.w;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(up + (i * kTileCols + m0 + g + 8 * h) * pitch + c * kK +
+                                                                     k * 32 + 8 * q);
+                    ua[0][i][h] = v.x, ua[0][i][2 + h] = v.y, ua[1][i][h] = v.z, ua[1][i][2 + h] = v.w;
                 }
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int row = nb + 8 * (g >> 1) + 2 * b + (g & 1);
-                uint32_t wq[Weight<T>::kPieces][4];
-                weights(load_eight<T, VB>(B + row * t.sb_row + k + 8 * q, row < n1 ? r - k - 8 * q : 0), wq);
-                float acc[4] = {};
-#pragma unroll
-                for (int i = 2; i >= 0; --i)
-#pragma unroll
-                    for (int k2 = Weight<T>::kPieces - 1; k2 >= 0; --k2)
-                        if (i + k2 <= 2)
-#pragma unroll
-                            for (int m = 0; m < 2; ++m) mma_bf16(acc, ua[m][i], wq[k2][2 * m], wq[k2][2 * m + 1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[b][e] += acc[e];
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (!live[h]) continue;
-            float *d = t.dst + col[h] * t.sdst + n;
+            float acc[4][4];
+            products<T>(acc, ua, [&](int b) {
+                return load_eight_smem(w + (8 * (g >> 1) + 2 * b + (g & 1)) * kPitch + k * 32 + 8 * q);
+            });
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) y[h].v[2 * b + e] += sum[b][2 * h + e];
+                for (int e = 0; e < 4; ++e) sum[b][e] += acc[b][e];
+        }
+        if (c + 1 < chunks) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    y[h].v[2 * b + e] += sum[b][2 * h + e];
+                    sum[b][2 * h + e] = 0.0f;
+                }
+            if (dst[h] == nullptr) continue;
+            float *d = dst[h] + n;
             if (VY && n + 8 <= n1) {
                 reinterpret_cast<float4 *>(d)[0] = reinterpret_cast<float4 *>(&y[h])[0];
                 reinterpret_cast<float4 *>(d)[1] = reinterpret_cast<float4 *>(&y[h])[1];
@@ -705,11 +768,18 @@ __global__ void __launch_bounds__(256) k_lora_expand(const __grid_constant__ Lor
                     if (n + e < n1) d[e] = y[h].v[e];
             }
         }
+        y[0] = next[0];
+        y[1] = next[1];
+        n += 64;
     }
 }
 
 size_t shrink_smem(int esz) { return static_cast<size_t>(kRing) * kRanks * kStageK * esz; }
-size_t expand_smem(int rank) { return static_cast<size_t>(3) * kTileCols * ((rank + 31) / 32 * 32 + 8) * 2; }
+template <typename T> size_t expand_smem(int rank) {
+    constexpr int kK = RowStage<T>::kK;
+    return static_cast<size_t>(kRing) * RowStage<T>::kValues * sizeof(T) +
+           static_cast<size_t>(3) * kTileCols * ((rank + kK - 1) / kK * kK + 8) * 2;
+}
 
 // A launch that may begin while the one before it ends (its kernel waits for it).
 template <typename K>
@@ -741,7 +811,7 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool 
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        const int ss = static_cast<int>(shrink_smem(sizeof(T))), es = static_cast<int>(expand_smem(Q4K_MAX_LORA_RANK));
+        const int ss = static_cast<int>(shrink_smem(sizeof(T))), es = static_cast<int>(expand_smem<T>(Q4K_MAX_LORA_RANK));
         for (auto *f : {k_lora_shrink<T, true, true>, k_lora_shrink<T, true, false>, k_lora_shrink<T, false, true>,
                         k_lora_shrink<T, false, false>})
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ss)) != cudaSuccess) return e;
@@ -762,8 +832,8 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool 
         e = launch_next(shrink, dim3(tiles, p.splits, chunks), 128, shrink_smem(sizeof(T)), p, s);
         if (e != cudaSuccess) return e;
     }
-    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 256, expand_smem(rank),
-                       p, s);
+    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 256,
+                       expand_smem<T>(rank), p, s);
 }
 
 // Whether every run of 8 values of every row is 16-byte aligned.
@@ -867,6 +937,9 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
 }
 
 // Workspace of the many-column path: number of tiles, tiles, order, u.
+#ifndef LORA_CTAS
+#define LORA_CTAS 512
+#endif
 struct LoraLayout {
     size_t tiles = 0, order = 0, u = 0, total = 0;
     int max_slots = 0, u_cols = 0, splits = 1;
@@ -884,7 +957,7 @@ LoraLayout lora_layout(const q4k_lora_task *tasks, int ntasks, int ncols) {
     }
     // K is split until there are two or three CTAs for each of the SMs, but not below four stages
     const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
-    while (L.splits < 16 && tiles * L.splits < 256 && K >= 2 * L.splits * 4 * kStageK) L.splits *= 2;
+    while (L.splits < 16 && tiles * L.splits < LORA_CTAS && K >= 2 * L.splits * 4 * kStageK) L.splits *= 2;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     L.tiles = 256;
     L.order = L.tiles + up(static_cast<size_t>(most_tiles(ncols, L.max_slots)) * sizeof(LoraTile));
