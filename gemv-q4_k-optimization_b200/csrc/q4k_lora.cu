@@ -26,7 +26,7 @@ struct LoraTask {
     const float *scales;
     int64_t sx, sbase, sdst, sa_slot, sa_row, sb_slot, sb_row;
     int K, nrows, slots, rank;
-    int u_off;  // first value of this task in a column's u
+    int u_off;  // first value of this task in a column's u (a multiple of 8)
 };
 
 // Columns of one adapter that are worked on together (many columns).
@@ -42,7 +42,7 @@ struct LoraParams {
     int *ntiles;
     LoraTile *tiles;
     int *order;   // columns sorted by adapter
-    float *u;     // splits x ncols x u_cols, in sorted order
+    uint16_t *u;  // three bf16 pieces of u: 3 x ncols x u_cols, in sorted order
     int u_cols, splits, max_slots, rows_per_cta;
 };
 
@@ -511,22 +511,27 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, int bytes
                  : "memory");
 }
 
-// Stage of A in shared memory: kRanks rows of kStageK values, as kStageK / 32
-// slabs of 32 (rows 32 * sizeof(T) apart: the eight rows and four eights of a
-// fragment load cover all banks).
+// Stage of the shrink's ring: kStageK values of kTileCols columns of x, and of
+// kRanks rows of A as kStageK / 32 slabs of 32. Pitches let the eight rows and
+// four eights of a fragment load meet different banks.
+constexpr int kXPitch = kStageK + 4;
 constexpr int kStageValues = kRanks * kStageK;
+template <typename T> constexpr size_t kShrinkStage = kTileCols * kXPitch * 4 + kStageValues * sizeof(T);
+constexpr int kMaxSplits = 8;  // CTAs that share a tile's K: a cluster
 
-// u of a tile's columns for kRanks ranks, over this CTA's share of K. Four
-// warps, 16 columns each: x goes from memory straight into MMA fragments
-// (lane t of a row takes eights of consecutive values; A is read in the same
-// order, so the sum is over the same pairs), A through shared memory.
+// u of a tile's columns for kRanks ranks. The cluster splits K; in a CTA four
+// pairs of warps take 16 columns each, a warp one half of every stage. x and A come through a ring; lane q of a row
+// takes eights of consecutive values of both, so the MMAs sum over the same
+// pairs whatever their order. The CTAs' sums meet over distributed shared
+// memory, and u leaves as the pieces that the expand's MMAs take.
 template <typename T, bool VX, bool VA>
-__global__ void __launch_bounds__(128) k_lora_shrink(const __grid_constant__ LoraParams P) {
+__global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ LoraParams P) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    T *stage = reinterpret_cast<T *>(smem_raw);
+    __shared__ const float *xcol[kTileCols];
+    cg::cluster_group cluster = cg::this_cluster();
     pdl_launch_dependents();
     pdl_wait();
-    if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;
+    if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;  // (the whole cluster, here and below)
     const LoraTile tile = P.tiles[blockIdx.x];
     int z = blockIdx.z, ti = 0;
     while (z >= (P.task[ti].rank + kRanks - 1) / kRanks) z -= (P.task[ti++].rank + kRanks - 1) / kRanks;
@@ -534,92 +539,114 @@ __global__ void __launch_bounds__(128) k_lora_shrink(const __grid_constant__ Lor
     const int a = slot_of(t, tile.slot), r = a < 0 ? 0 : rank_of(t, a), r0 = z * kRanks;
     if (r0 >= r) return;
     const int nr = min(kRanks, r - r0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, q = lane & 3;
+    const int g = lane >> 2, q = lane & 3, m0 = (warp & 3) * 16, half = warp >> 2;
+    if (tid < tile.count) xcol[tid] = t.x + P.order[tile.first + tid] * t.sx;
+    __syncthreads();
     // this CTA's share of K: whole stages
     const int stages = (t.K + kStageK - 1) / kStageK, per = (stages + P.splits - 1) / P.splits;
     const int s0 = min(stages, static_cast<int>(blockIdx.y) * per), s1 = min(stages, s0 + per);
-    const bool busy = warp * 16 < tile.count;
-    const float *xr[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = warp * 16 + g + 8 * h;
-        xr[h] = i < tile.count ? t.x + P.order[tile.first + i] * t.sx : nullptr;
-    }
+    const bool busy = m0 < tile.count;
     const T *A = static_cast<const T *>(t.A) + a * t.sa_slot + r0 * t.sa_row;
     auto fill = [&](int s) {
-        T *to = stage + (s % kRing) * kStageValues;
+        float *xs = reinterpret_cast<float *>(smem_raw + (s % kRing) * kShrinkStage<T>);
+        T *as = reinterpret_cast<T *>(xs + kTileCols * kXPitch);
         if (s < s1) {
+            const int k0 = s * kStageK;
+            if constexpr (VX) {
+                const int k = tid % 16 * 4, left = min(4, t.K - k0 - k);
+                for (int row = tid / 16; row < tile.count; row += 16)
+                    cp_async16(xs + row * kXPitch + k, left > 0 ? xcol[row] + k0 + k : xcol[row], left > 0 ? left * 4 : 0);
+            } else {
+                for (int i = tid; i < tile.count * kStageK; i += 256) {
+                    const int row = i / kStageK, k = i % kStageK;
+                    xs[row * kXPitch + k] = k0 + k < t.K ? xcol[row][k0 + k] : 0.0f;
+                }
+            }
             if constexpr (VA) {
                 constexpr int E = 16 / sizeof(T), C = kStageK / E;  // values per copy, copies per row
-                for (int i = tid; i < kRanks * C; i += 128) {
-                    const int row = i / C, k = (i - row * C) * E, left = row < nr ? min(E, t.K - s * kStageK - k) : 0;
-                    const bool some = left > 0;
-                    cp_async16(to + ((k / 32) * kRanks + row) * 32 + k % 32, some ? A + row * t.sa_row + s * kStageK + k : A,
+                const int k = tid % C * E, left = min(E, t.K - k0 - k);
+                for (int row = tid / C; row < kRanks; row += 256 / C) {
+                    const bool some = left > 0 && row < nr;
+                    cp_async16(as + ((k / 32) * kRanks + row) * 32 + k % 32, some ? A + row * t.sa_row + k0 + k : A,
                                some ? left * static_cast<int>(sizeof(T)) : 0);
                 }
             } else {
-                for (int i = tid; i < kRanks * kStageK; i += 128) {
+                for (int i = tid; i < kRanks * kStageK; i += 256) {
                     const int row = i / kStageK, k = i % kStageK;
-                    to[((k / 32) * kRanks + row) * 32 + k % 32] =
-                        row < nr && s * kStageK + k < t.K ? A[row * t.sa_row + s * kStageK + k] : T(0.0f);
+                    as[((k / 32) * kRanks + row) * 32 + k % 32] = row < nr && k0 + k < t.K ? A[row * t.sa_row + k0 + k] : T(0.0f);
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto load_x = [&](Eight<float> (&x)[2], int k) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[h] = load_eight<float, VX>(xr[h] + k + 8 * q, xr[h] != nullptr ? t.K - k - 8 * q : 0);
-    };
     float sum[8][4] = {};
-    Eight<float> x[2];
 #pragma unroll
     for (int i = 0; i < kRing - 1; ++i) fill(s0 + i);
-    if (busy && s0 < s1) load_x(x, s0 * kStageK);
     for (int s = s0; s < s1; ++s) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
         __syncthreads();  // stage s has come, and stage s - 1 may be written again
         fill(s + kRing - 1);
         if (!busy) continue;
-        const T *w = stage + (s % kRing) * kStageValues;
+        const float *xs = reinterpret_cast<const float *>(smem_raw + (s % kRing) * kShrinkStage<T>);
+        const T *as = reinterpret_cast<const T *>(xs + kTileCols * kXPitch);
+        uint32_t xa[2][3][4];  // [MMA][piece][operand registers]
 #pragma unroll
-        for (int half = 0; half < kStageK / 32; ++half) {
-            uint32_t xa[2][3][4];  // [MMA][piece][operand registers]
+        for (int h = 0; h < 2; ++h) {
+            // (rows behind the tile's columns hold anything: an MMA keeps rows apart)
+            const Eight<float> x = load_eight_smem(xs + (m0 + g + 8 * h) * kXPitch + half * 32 + 8 * q);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < 4; ++i) {
+                uint32_t p[3];
+                pieces(x.v[2 * i], x.v[2 * i + 1], p);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t p[3];
-                    pieces(x[h].v[2 * i], x[h].v[2 * i + 1], p);
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) xa[i / 2][k][(i % 2) * 2 + h] = p[k];
-                }
-            const int k = s * kStageK + half * 32 + 32;
-            if (half == 0 || s + 1 < s1) load_x(x, k);  // (zeros behind K)
-#pragma unroll
-            for (int n = 0; n < 8; n += 4) {
-                if (n * 8 >= nr) break;
-                float acc[4][4];
-                products<T>(acc, xa, [&](int b) { return load_eight_smem(w + (half * kRanks + (n + b) * 8 + g) * 32 + 8 * q); });
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[n + b][e] += acc[b][e];
+                for (int k = 0; k < 3; ++k) xa[i / 2][k][(i % 2) * 2 + h] = p[k];
             }
         }
-    }
-    if (!busy) return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = warp * 16 + g + 8 * h;
-        if (i >= tile.count) continue;
-        float *u = P.u + (static_cast<int64_t>(blockIdx.y) * P.ncols + tile.first + i) * P.u_cols + t.u_off + r0;
+        for (int n = 0; n < 8; n += 4) {
+            if (n * 8 >= nr) break;
+            float acc[4][4];
+            products<T>(acc, xa, [&](int b) { return load_eight_smem(as + (half * kRanks + (n + b) * 8 + g) * 32 + 8 * q); });
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[n + b][e] += acc[b][e];
+        }
+    }
+    // the halves' sums, [half][column][rank], over the ring
+    constexpr int kPitch = kRanks + 4;
+    float *part = reinterpret_cast<float *>(smem_raw);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    if (busy)
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (n * 8 + 2 * q + e < nr) u[n * 8 + 2 * q + e] = sum[n][2 * h + e];
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2 *>(part + (half * kTileCols + m0 + g + 8 * h) * kPitch + n * 8 + 2 * q) =
+                    make_float2(sum[n][2 * h], sum[n][2 * h + 1]);
+    cluster.sync();
+    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
+    const int pairs = (nr + 7) / 8 * 4;  // (whole eights: zeros behind the rank)
+    for (int i = blockIdx.y * 256 + tid; i < tile.count * (kRanks / 2); i += P.splits * 256) {
+        const int col = i / (kRanks / 2), k = i % (kRanks / 2);
+        if (k >= pairs) continue;
+        float2 v = make_float2(0.0f, 0.0f);
+        for (int c = 0; c < P.splits; ++c) {
+            const float *from = cluster.map_shared_rank(part, c) + col * kPitch + 2 * k;
+            const float2 w0 = *reinterpret_cast<const float2 *>(from);
+            const float2 w1 = *reinterpret_cast<const float2 *>(from + kTileCols * kPitch);
+            v.x += w0.x + w1.x;
+            v.y += w0.y + w1.y;
+        }
+        uint32_t p[3];
+        pieces(2 * k < nr ? v.x * scale : 0.0f, 2 * k + 1 < nr ? v.y * scale : 0.0f, p);
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            *reinterpret_cast<uint32_t *>(P.u + (static_cast<int64_t>(e) * P.ncols + tile.first + col) * P.u_cols + t.u_off + r0 +
+                                          2 * k) = p[e];
     }
+    cluster.sync();  // no CTA leaves while another may still read its part
 }
 
 // dst of a tile's columns for a range of rows. Eight warps: 16 columns each, two
@@ -681,6 +708,12 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // the pieces of u come with the first stage (zeros behind the rank)
+    for (int i = tid; i < 3 * tile.count * (rp / 8); i += 256) {
+        const int k = i % (rp / 8) * 8, pc = i / (rp / 8), piece = pc / tile.count, col = pc - piece * tile.count;
+        const uint16_t *u = P.u + (static_cast<int64_t>(piece) * P.ncols + tile.first + col) * P.u_cols + t.u_off;
+        cp_async16(up + (piece * kTileCols + col) * pitch + k, k < r ? u + k : u, k < r ? 16 : 0);
+    }
 #pragma unroll
     for (int i = 0; i < kRing - 1; ++i) fill(i);
 
@@ -702,20 +735,6 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ 
     };
     Eight<float> y[2];
     load_base(y, n);
-    const float scale = t.scales != nullptr ? t.scales[a] : 1.0f;
-    for (int i = tid; i < tile.count * (rp / 2); i += 256) {
-        const int col = i / (rp / 2), k = (i - col * (rp / 2)) * 2;
-        float v[2] = {0.0f, 0.0f};
-        const float *u = P.u + (static_cast<int64_t>(tile.first) + col) * P.u_cols + t.u_off + k;
-        for (int s = 0; s < P.splits; ++s)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (k + e < r) v[e] += u[static_cast<int64_t>(s) * P.ncols * P.u_cols + e];
-        uint32_t p[3];
-        pieces(v[0] * scale, v[1] * scale, p);
-#pragma unroll
-        for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t *>(up + (e * kTileCols + col) * pitch + k) = p[e];
-    }
     float sum[4][4] = {};
     for (int s = 0, c = 0; s < stages; ++s, c = c + 1 == chunks ? 0 : c + 1) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
@@ -774,7 +793,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ 
     }
 }
 
-size_t shrink_smem(int esz) { return static_cast<size_t>(kRing) * kRanks * kStageK * esz; }
+template <typename T> constexpr size_t kShrinkSmem = kRing * kShrinkStage<T>;
 template <typename T> size_t expand_smem(int rank) {
     constexpr int kK = RowStage<T>::kK;
     return static_cast<size_t>(kRing) * RowStage<T>::kValues * sizeof(T) +
@@ -783,17 +802,21 @@ template <typename T> size_t expand_smem(int rank) {
 
 // A launch that may begin while the one before it ends (its kernel waits for it).
 template <typename K>
-cudaError_t launch_next(K *fn, dim3 grid, int threads, size_t smem, const LoraParams &p, cudaStream_t s) {
+cudaError_t launch_next(K *fn, dim3 grid, int cluster_y, int threads, size_t smem, const LoraParams &p, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = cluster_y;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster_y > 0 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
@@ -811,7 +834,7 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool 
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        const int ss = static_cast<int>(shrink_smem(sizeof(T))), es = static_cast<int>(expand_smem<T>(Q4K_MAX_LORA_RANK));
+        const int ss = static_cast<int>(kShrinkSmem<T>), es = static_cast<int>(expand_smem<T>(Q4K_MAX_LORA_RANK));
         for (auto *f : {k_lora_shrink<T, true, true>, k_lora_shrink<T, true, false>, k_lora_shrink<T, false, true>,
                         k_lora_shrink<T, false, false>})
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ss)) != cudaSuccess) return e;
@@ -829,10 +852,10 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool 
         rows = std::max(rows, static_cast<unsigned>(p.task[i].nrows));
     }
     if (chunks > 0) {
-        e = launch_next(shrink, dim3(tiles, p.splits, chunks), 128, shrink_smem(sizeof(T)), p, s);
+        e = launch_next(shrink, dim3(tiles, p.splits, chunks), p.splits, 256, kShrinkSmem<T>, p, s);
         if (e != cudaSuccess) return e;
     }
-    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 256,
+    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 0, 256,
                        expand_smem<T>(rank), p, s);
 }
 
@@ -938,7 +961,7 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
 
 // Workspace of the many-column path: number of tiles, tiles, order, u.
 #ifndef LORA_CTAS
-#define LORA_CTAS 512
+#define LORA_CTAS 256
 #endif
 struct LoraLayout {
     size_t tiles = 0, order = 0, u = 0, total = 0;
@@ -952,17 +975,17 @@ LoraLayout lora_layout(const q4k_lora_task *tasks, int ntasks, int ncols) {
     for (int i = 0; i < ntasks; ++i) {
         if (tasks[i].nrows == 0) continue;
         L.max_slots = std::max(L.max_slots, tasks[i].slots);
-        L.u_cols += tasks[i].rank;
+        L.u_cols += (tasks[i].rank + 7) / 8 * 8;
         K = std::max(K, tasks[i].K);
     }
-    // K is split until there are two or three CTAs for each of the SMs, but not below four stages
+    // K is split until there are about LORA_CTAS CTAs (two or three for each SM), but not below four stages
     const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
-    while (L.splits < 16 && tiles * L.splits < LORA_CTAS && K >= 2 * L.splits * 4 * kStageK) L.splits *= 2;
+    L.splits = static_cast<int>(std::max<int64_t>(1, std::min({int64_t(kMaxSplits), LORA_CTAS / tiles, K / (4 * kStageK)})));
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     L.tiles = 256;
     L.order = L.tiles + up(static_cast<size_t>(most_tiles(ncols, L.max_slots)) * sizeof(LoraTile));
     L.u = L.order + up(static_cast<size_t>(ncols) * 4);
-    L.total = L.u + up(static_cast<size_t>(L.splits) * ncols * L.u_cols * 4);
+    L.total = L.u + up(static_cast<size_t>(3) * ncols * L.u_cols * 2);
     return L;
 }
 
@@ -996,7 +1019,7 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
         d = {t.x, t.base, t.dst, t.A, t.B, t.ranks, t.scales, t.stride_col_x, t.stride_col_base, t.stride_col_dst,
              t.stride_a_slot, t.stride_a_row, t.stride_b_slot, t.stride_b_row, static_cast<int>(t.K),
              static_cast<int>(t.nrows), none || t.rank == 0 ? 0 : t.slots, t.rank, p.u_cols};
-        p.u_cols += t.rank;
+        p.u_cols += (t.rank + 7) / 8 * 8;
     }
     if (n == 0) return Q4K_OK;
     p.ids = ids;
@@ -1007,7 +1030,7 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
         p.ntiles = reinterpret_cast<int *>(ws);
         p.tiles = reinterpret_cast<LoraTile *>(ws + L.tiles);
         p.order = reinterpret_cast<int *>(ws + L.order);
-        p.u = reinterpret_cast<float *>(ws + L.u);
+        p.u = reinterpret_cast<uint16_t *>(ws + L.u);
         p.splits = L.splits;
         p.max_slots = L.max_slots;
         // rows per expand CTA: few enough for several CTAs per SM
