@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 from pathlib import Path
 from typing import Sequence
 
@@ -174,11 +175,11 @@ def lib() -> ctypes.CDLL:
             "q4k_ipc_close": (None, [_P]),
             "q4k_batch_ex_kernel": (_I, [TXP, _I, _I, _I]),
             "q4k_batch_persistent_kernel": (_I, [TP, _I, _I, _I]),
-            "q4k_lora_workspace_bytes": (_SZ, [ctypes.POINTER(LoraTask), _I, _I]),
-            "q4k_lora_batch": (None, [ctypes.POINTER(LoraTask), _I, _I, _P, _P, _SZ, _P]),
-            "q4k_rope_multi": (None, [ctypes.POINTER(RopeTensor), _I, _I, _I, _I, _P, _I64, _P, ctypes.POINTER(_I),
-                                      _I, _I, _I, ctypes.c_float, _I, _P]),
-            "q4k_logits_process": (None, [ctypes.POINTER(LogitsArgs), _I, _P]),
+            # (structs as void *: ctypes structures and packed bytes alike)
+            "q4k_lora_workspace_bytes": (_SZ, [_P, _I, _I]),
+            "q4k_lora_batch": (None, [_P, _I, _I, _P, _P, _SZ, _P]),
+            "q4k_rope_multi": (None, [_P, _I, _I, _I, _I, _P, _I64, _P, _P, _I, _I, _I, ctypes.c_float, _I, _P]),
+            "q4k_logits_process": (None, [_P, _I, _P]),
             "q4k_timeline_bytes": (_SZ, []),
             "q4k_timeline_read": (None, [_P, _SZ, ctypes.POINTER(_I)]),
             "q4k_timeline_reset": (None, []),
@@ -600,91 +601,106 @@ ROPE_LAYOUTS = {"half": 0, "adjacent": 1}
 ROPE_ORDERS = {"blocks": 0, "interleaved": 1}
 
 
+# The structs above as the wrappers fill them: packed bytes cost a tenth of a
+# ctypes structure, and a small call's time is the host's.
+_PACK_LORA = struct.Struct("7Q9q3i4x")
+_PACK_ROPE = struct.Struct("2Q4qi4x")
+_PACK_LOGITS = struct.Struct("2Q3q3Q2q3Qq2Qqi4x2Q")
+_types: dict = {}  # torch dtype -> Q4K_TYPE_*
+
+
 def _type_of(dtype) -> int:
-    import torch
-    t = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}.get(dtype)
+    if not _types:
+        import torch
+        _types.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    t = _types.get(dtype)
     if t is None:
         raise Q4KError(1, f"type {dtype} is not float32, float16 or bfloat16")
     return t
 
 
-def _dense(t, name: str, ndim: int, dtype, device):
-    """t, checked: on `device`, of `dtype` (None: any) and `ndim` dimensions, the last one contiguous."""
-    if t.dim() != ndim or t.device != device or (dtype is not None and t.dtype != dtype):
-        raise Q4KError(1, f"{name}: {ndim}-d {dtype or 'tensor'} on {device} expected, got {tuple(t.shape)} "
+def _dense(t, name: str, ndim: int, dtype, device: int):
+    """t, checked: on CUDA device `device`, of `dtype` (None: any) and `ndim` dimensions, the last one contiguous."""
+    if t.dim() != ndim or t.get_device() != device or (dtype is not None and t.dtype != dtype):
+        raise Q4KError(1, f"{name}: {ndim}-d {dtype or 'tensor'} on cuda:{device} expected, got {tuple(t.shape)} "
                           f"{t.dtype} on {t.device}")
-    if ndim and t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.stride()[-1] != 1 and t.shape[-1] > 1:
         raise Q4KError(1, f"{name}: the last dimension is not contiguous")
     return t
 
 
-def _flat(t, name: str, dtype, n: int, device) -> int | None:
-    """Address of a contiguous 1-d tensor of n values (None stays None)."""
+def _flat(t, name: str, dtype, n: int, device: int) -> int:
+    """Address of a contiguous 1-d tensor of n values (None: 0)."""
     if t is None:
-        return None
-    if t.shape != (n,):
-        raise Q4KError(1, f"{name}: {n} values expected, got {tuple(t.shape)}")
-    return _dense(t, name, 1, dtype, device).data_ptr()
+        return 0
+    if t.get_device() != device or t.dtype != dtype or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
+        raise Q4KError(1, f"{name}: {n} contiguous values of {dtype} on cuda:{device} expected, got {tuple(t.shape)} "
+                          f"{t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
-def _on_cuda(t, name: str):
+def _cuda_index(t, name: str) -> int:
     if not t.is_cuda:
         raise Q4KError(1, f"{name}: not a CUDA tensor (there is no CPU fallback)")
-    return t.device
+    return t.get_device()
 
 
-def _new(shape, dtype, device, stream):
-    """An uninitialised tensor that belongs to the stream the call runs on."""
+def _new(like, shape, dtype, stream):
+    """An uninitialised tensor on like's device that belongs to the stream the call runs on."""
     import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
+        stream = torch.cuda.ExternalStream(stream, device=like.device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _call_on(device, stream, fn, *args) -> int:
+def _call_on(device: int, stream, fn, *args) -> int:
     """fn(*args, stream) with the tensors' device current; stream None: that device's current one."""
     import torch
-    s = torch.cuda.current_stream(device).cuda_stream if stream is None else _stream(stream)
-    if device.index == torch.cuda.current_device():
+    s = torch._C._cuda_getCurrentRawStream(device) if stream is None else _stream(stream)
+    if device == torch.cuda.current_device():
         return fn(*args, s)
     with torch.cuda.device(device):
         return fn(*args, s)
 
 
-def _lora_fill(t: LoraTask, it: dict, stream):
-    """One q4k_lora_task from a dict; returns (output, ncols, device)."""
+def _lora_pack(x, A, B, base, ranks, scales, out, stream):
+    """One q4k_lora_task as bytes; returns (bytes, output, ncols, device index, type)."""
     import torch
-    x, A, B, base, out = it["x"], it["A"], it["B"], it.get("base"), it.get("out")
-    dev = _on_cuda(x, "x")
+    f32 = torch.float32
+    dev = _cuda_index(x, "x")
     if x.dim() == 1:
         x = x.unsqueeze(0)
-    ncols, K = _dense(x, "x", 2, torch.float32, dev).shape
+    ncols, K = _dense(x, "x", 2, f32, dev).shape
     slots, rank, ka = _dense(A, "A", 3, None, dev).shape
     sb, nrows, rb = _dense(B, "B", 3, A.dtype, dev).shape
     if ka != K or sb != slots or rb != rank:
         raise Q4KError(1, f"A {tuple(A.shape)} and B {tuple(B.shape)} do not fit x {tuple(x.shape)}")
-    t.type = _type_of(A.dtype)
     if out is None:
-        out = _new((ncols, nrows), torch.float32, dev, stream)
-    o = out.unsqueeze(0) if out.dim() == 1 else out
-    if _dense(o, "out", 2, torch.float32, dev).shape != (ncols, nrows):
-        raise Q4KError(1, f"out {tuple(out.shape)}: ({ncols}, {nrows}) expected")
+        out = _new(x, (ncols, nrows), None, stream)
+        o = out
+    else:
+        o = out.unsqueeze(0) if out.dim() == 1 else out
+        if _dense(o, "out", 2, f32, dev).shape != (ncols, nrows):
+            raise Q4KError(1, f"out {tuple(out.shape)}: ({ncols}, {nrows}) expected")
+    bp = bs = 0
     if base is not None:
         b = base.unsqueeze(0) if base.dim() == 1 else base
-        if _dense(b, "base", 2, torch.float32, dev).shape != (ncols, nrows):
+        if _dense(b, "base", 2, f32, dev).shape != (ncols, nrows):
             raise Q4KError(1, f"base {tuple(base.shape)}: ({ncols}, {nrows}) expected")
-        t.base, t.stride_col_base = b.data_ptr(), b.stride(0)
-    t.x, t.A, t.B, t.dst = x.data_ptr(), A.data_ptr(), B.data_ptr(), o.data_ptr()
-    t.ranks = _flat(it.get("ranks"), "ranks", torch.int32, slots, dev)
-    t.scales = _flat(it.get("scales"), "scales", torch.float32, slots, dev)
-    t.K, t.nrows, t.slots, t.rank = K, nrows, slots, rank
-    t.stride_col_x, t.stride_col_dst = x.stride(0), o.stride(0)
-    t.stride_a_slot, t.stride_a_row = A.stride(0), A.stride(1)
-    t.stride_b_slot, t.stride_b_row = B.stride(0), B.stride(1)
-    return out, ncols, dev
+        bp, bs = b.data_ptr(), b.stride()[0]
+    sa, sbs = A.stride(), B.stride()
+    kind = _type_of(A.dtype)
+    buf = _PACK_LORA.pack(x.data_ptr(), bp, o.data_ptr(), A.data_ptr(), B.data_ptr(),
+                          _flat(ranks, "ranks", torch.int32, slots, dev), _flat(scales, "scales", f32, slots, dev),
+                          K, nrows, x.stride()[0], bs, o.stride()[0], sa[0], sa[1], sbs[0], sbs[1], slots, rank, kind)
+    return buf, out, ncols, dev
+
+
+def _lora_pack_item(it: dict, stream):
+    return _lora_pack(it["x"], it["A"], it["B"], it.get("base"), it.get("ranks"), it.get("scales"), it.get("out"), stream)
 
 
 def make_lora_tasks(items: Sequence):
@@ -692,30 +708,28 @@ def make_lora_tasks(items: Sequence):
     A (slots, rank, K) and B (slots, nrows, rank) of one type (fp32, fp16 or bf16), out
     (ncols, nrows) and optionally base (fp32 like out, may be out itself), ranks (slots
     int32) and scales (slots fp32).  The tensors must outlive the array."""
-    arr = (LoraTask * len(items))()
-    for t, it in zip(arr, items):
-        if it.get("out") is None:
-            raise Q4KError(1, "make_lora_tasks: an item has no out")
-        _lora_fill(t, it, None)
-    return arr
+    if any(it.get("out") is None for it in items):
+        raise Q4KError(1, "make_lora_tasks: an item has no out")
+    return (LoraTask * len(items)).from_buffer_copy(b"".join(_lora_pack_item(it, None)[0] for it in items))
 
 
-def _lora_call(arr, ncols: int, ids, dev, ws, stream) -> None:
+def _lora_call(tasks, n: int, ncols: int, ids, dev: int, ws, stream) -> None:
     import torch
     idp = _flat(ids, "ids", torch.int32, ncols, dev)
-    fn, n = lib().q4k_lora_batch, len(arr)
-    st = _call_on(dev, stream, fn, arr, n, ncols, idp, ws.ptr if ws is not None else None,
+    fn = lib().q4k_lora_batch
+    st = _call_on(dev, stream, fn, tasks, n, ncols, idp, ws.ptr if ws is not None else None,
                   ws.nbytes if ws is not None else 0)
     if st == 5:
-        need = int(lib().q4k_lora_workspace_bytes(arr, n, ncols))
+        need = int(lib().q4k_lora_workspace_bytes(tasks, n, ncols))
         if ws is not None:
             ws.ensure(need)
             p = ws.ptr
         else:  # scratch of this call's own, so calls on several streams or in several graphs share nothing
-            scratch = _new((need,), torch.uint8, dev, stream)
+            scratch = _new(ids, (need,), torch.uint8, stream)
             p = scratch.data_ptr()
-        st = _call_on(dev, stream, fn, arr, n, ncols, idp, p, need)
-    _check(st)
+        st = _call_on(dev, stream, fn, tasks, n, ncols, idp, p, need)
+    if st:
+        _check(st)
 
 
 def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
@@ -725,23 +739,23 @@ def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
     adapter, out[j] = base[j]).  tasks: dicts as for make_lora_tasks (out may be left
     out), returns the list of outputs; or its array, returns None."""
     if isinstance(tasks, ctypes.Array):
-        _lora_call(tasks, ids.shape[0], ids, _on_cuda(ids, "ids"), ws, stream)
+        _lora_call(tasks, len(tasks), ids.shape[0], ids, _cuda_index(ids, "ids"), ws, stream)
         return None
     if len(tasks) == 0:
         return []
-    arr = (LoraTask * len(tasks))()
-    got = [_lora_fill(t, it, stream) for t, it in zip(arr, tasks)]
-    if any(g[1:] != got[0][1:] for g in got):
-        raise Q4KError(1, "the tasks' columns or devices differ")
-    _lora_call(arr, got[0][1], ids, got[0][2], ws, stream)
-    return [g[0] for g in got]
+    got = [_lora_pack_item(it, stream) for it in tasks]
+    ncols, dev = got[0][2:]
+    for g in got:
+        if g[2] != ncols or g[3] != dev:
+            raise Q4KError(1, "the tasks' columns or devices differ")
+    _lora_call(b"".join([g[0] for g in got]), len(got), ncols, ids, dev, ws, stream)
+    return [g[1] for g in got]
 
 
 def lora_add(x, A, B, ids, base=None, ranks=None, scales=None, out=None, ws: Workspace | None = None, stream=None):
     """lora_batch for one projection; returns (ncols, nrows) fp32."""
-    t = (LoraTask * 1)()
-    out, ncols, dev = _lora_fill(t[0], dict(x=x, A=A, B=B, base=base, ranks=ranks, scales=scales, out=out), stream)
-    _lora_call(t, ncols, ids, dev, ws, stream)
+    buf, out, ncols, dev = _lora_pack(x, A, B, base, ranks, scales, out, stream)
+    _lora_call(buf, 1, ncols, ids, dev, ws, stream)
     return out
 
 
@@ -766,35 +780,43 @@ def rope_multi(x, pos, inv_freq, sections, layout: str = "half", order: str = "b
     `dtype`: fp32, fp16 or bf16).  Returns out."""
     import torch
     single = not isinstance(x, (list, tuple))
-    xs = [x] if single else list(x)
-    if layout not in ROPE_LAYOUTS or order not in ROPE_ORDERS:
+    xs = [x] if single else x
+    lay, order_id = ROPE_LAYOUTS.get(layout), ROPE_ORDERS.get(order)
+    if lay is None or order_id is None:
         raise Q4KError(1, f"layout {layout!r} / order {order!r}")
     outs = [None] * len(xs) if out is None else [out] if single else list(out)
     if not 1 <= len(xs) <= 4 or len(outs) != len(xs):
         raise Q4KError(1, "1 to 4 tensors, and as many outputs")
-    dev = _on_cuda(xs[0], "x")
-    ncols, _, dim = xs[0].shape if xs[0].dim() == 3 else (0, 0, 0)
+    f32 = torch.float32
+    dev = _cuda_index(xs[0], "x")
+    ncols, _, dim = _dense(xs[0], "x", 3, f32, dev).shape
     if dtype is None:
-        dtype = outs[0].dtype if outs[0] is not None else torch.float32
-    arr = (RopeTensor * len(xs))()
-    for i, (t, v) in enumerate(zip(arr, xs)):
-        _dense(v, "x", 3, torch.float32, dev)
-        if outs[i] is None:
-            outs[i] = _new(v.shape, dtype, dev, stream)
-        o = _dense(outs[i], "out", 3, dtype, dev)
-        if o.shape != v.shape or v.shape[0] != ncols or v.shape[2] != dim:
-            raise Q4KError(1, f"x {tuple(v.shape)}, out {tuple(o.shape)}: ({ncols}, heads, {dim}) expected")
-        t.x, t.dst, t.heads = v.data_ptr(), o.data_ptr(), v.shape[1]
-        t.stride_col_x, t.stride_head_x = v.stride(0), v.stride(1)
-        t.stride_col_dst, t.stride_head_dst = o.stride(0), o.stride(1)
+        dtype = outs[0].dtype if outs[0] is not None else f32
+    kind = _type_of(dtype)
+    packed = []
+    for i, v in enumerate(xs):
+        if i:
+            _dense(v, "x", 3, f32, dev)
+        c, heads, d = shape = v.shape
+        if c != ncols or d != dim:
+            raise Q4KError(1, f"x {tuple(shape)}: ({ncols}, heads, {dim}) expected")
+        o = outs[i]
+        if o is None:
+            o = outs[i] = _new(v, shape, dtype, stream)
+        elif _dense(o, "out", 3, dtype, dev).shape != shape:
+            raise Q4KError(1, f"out {tuple(o.shape)}: {tuple(shape)} expected")
+        sv, so = v.stride(), o.stride()
+        packed.append(_PACK_ROPE.pack(v.data_ptr(), o.data_ptr(), sv[0], sv[1], so[0], so[1], heads))
     _dense(pos, "pos", 2, torch.int32, dev)
-    _dense(inv_freq, "inv_freq", 1, torch.float64, dev)
-    if pos.shape != (len(sections), ncols):
-        raise Q4KError(1, f"pos {tuple(pos.shape)}: ({len(sections)}, {ncols}) expected")
-    sect = (_I * len(sections))(*sections)
-    _check(_call_on(dev, stream, lib().q4k_rope_multi, arr, len(xs), ncols, dim, 2 * inv_freq.shape[0],
-                    pos.data_ptr(), pos.stride(0), inv_freq.data_ptr(), sect, len(sections), ROPE_ORDERS[order],
-                    ROPE_LAYOUTS[layout], scale, _type_of(dtype)))
+    n = len(sections)
+    if pos.shape != (n, ncols):
+        raise Q4KError(1, f"pos {tuple(pos.shape)}: ({n}, {ncols}) expected")
+    half = inv_freq.shape[0]
+    st = _call_on(dev, stream, lib().q4k_rope_multi, b"".join(packed), len(xs), ncols, dim, 2 * half, pos.data_ptr(),
+                  pos.stride()[0], _flat(inv_freq, "inv_freq", torch.float64, half, dev), struct.pack(f"{n}i", *sections),
+                  n, order_id, lay, scale, kind)
+    if st:
+        _check(st)
     return outs[0] if single else outs
 
 
@@ -809,48 +831,54 @@ def logits_process(logits, history=None, history_len=None, penalties=None, bias_
     pick=True (out, token, lse): the lowest index of the largest value (-1: nothing left) and
     log(sum(exp)) of every column."""
     import torch
-    dev = _on_cuda(logits, "logits")
+    i32, f32 = torch.int32, torch.float32
+    dev = _cuda_index(logits, "logits")
     lg = logits.unsqueeze(0) if logits.dim() == 1 else logits
-    ncols, nvocab = _dense(lg, "logits", 2, torch.float32, dev).shape
+    ncols, nvocab = _dense(lg, "logits", 2, f32, dev).shape
     if out is None:
-        out = _new(logits.shape, torch.float32, dev, stream)
-    o = out.unsqueeze(0) if out.dim() == 1 else out
-    if _dense(o, "out", 2, torch.float32, dev).shape != lg.shape:
-        raise Q4KError(1, f"out {tuple(out.shape)}: {tuple(logits.shape)} expected")
-    if (history is None) != (penalties is None) or (history is None and history_len is not None):
-        raise Q4KError(1, "history and penalties go together")
-    if (bias_tokens is None) != (bias_values is None) or (bias_tokens is None) != (bias_offsets is None):
-        raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
-    if mask is None and mask_rows is not None:
-        raise Q4KError(1, "mask_rows without a mask")
-    a = LogitsArgs()
-    a.logits, a.dst, a.nvocab, a.stride_col, a.stride_col_dst = lg.data_ptr(), o.data_ptr(), nvocab, lg.stride(0), \
-        o.stride(0)
+        out = _new(lg, logits.shape, None, stream)
+        o = out.unsqueeze(0) if out.dim() == 1 else out
+    else:
+        o = out.unsqueeze(0) if out.dim() == 1 else out
+        if _dense(o, "out", 2, f32, dev).shape != lg.shape:
+            raise Q4KError(1, f"out {tuple(out.shape)}: {tuple(logits.shape)} expected")
+    hp = lp = pp = hmax = hs = 0
     if history is not None:
-        if history.shape[0] != ncols:
-            raise Q4KError(1, f"history {tuple(history.shape)}: {ncols} rows expected")
-        a.history = _dense(history, "history", 2, torch.int32, dev).data_ptr()
-        a.max_history, a.stride_history = history.shape[1], history.stride(0)
-        a.history_len = _flat(history_len, "history_len", torch.int32, ncols, dev)
-        if penalties.shape != (ncols, 3) or not penalties.is_contiguous():
+        hrows, hmax = _dense(history, "history", 2, i32, dev).shape
+        if penalties is None or hrows != ncols:
+            raise Q4KError(1, f"history {tuple(history.shape)}: {ncols} rows, with penalties, expected")
+        if _dense(penalties, "penalties", 2, f32, dev).shape != (ncols, 3) or not penalties.is_contiguous():
             raise Q4KError(1, f"penalties {tuple(penalties.shape)}: ({ncols}, 3) contiguous expected")
-        a.penalties = _dense(penalties, "penalties", 2, torch.float32, dev).data_ptr()
+        hp, lp, pp = history.data_ptr(), _flat(history_len, "history_len", i32, ncols, dev), penalties.data_ptr()
+        hs = history.stride()[0]
+    elif penalties is not None or history_len is not None:
+        raise Q4KError(1, "history and penalties go together")
+    bt = bv = bo = nb = 0
     if bias_tokens is not None:
-        a.n_bias = bias_tokens.shape[0]
-        a.bias_tokens = _flat(bias_tokens, "bias_tokens", torch.int32, a.n_bias, dev)
-        a.bias_values = _flat(bias_values, "bias_values", torch.float32, a.n_bias, dev)
-        a.bias_offsets = _flat(bias_offsets, "bias_offsets", torch.int32, ncols + 1, dev)
+        if bias_values is None or bias_offsets is None:
+            raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
+        nb = bias_tokens.shape[0]
+        bt, bv = _flat(bias_tokens, "bias_tokens", i32, nb, dev), _flat(bias_values, "bias_values", f32, nb, dev)
+        bo = _flat(bias_offsets, "bias_offsets", i32, ncols + 1, dev)
+    elif bias_values is not None or bias_offsets is not None:
+        raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
+    mp = mr = ms = nm = 0
     if mask is not None:
-        _dense(mask, "mask", 2, None, dev)
-        if mask.dtype not in (torch.int32, torch.uint32) or mask.shape[1] != (nvocab + 31) // 32:
+        nm, words = _dense(mask, "mask", 2, None, dev).shape
+        if mask.dtype not in (i32, torch.uint32) or words != (nvocab + 31) // 32:
             raise Q4KError(1, f"mask {tuple(mask.shape)} {mask.dtype}: (masks, {(nvocab + 31) // 32}) int32 expected")
-        a.mask, a.n_masks, a.stride_mask = mask.data_ptr(), mask.shape[0], mask.stride(0)
-        a.mask_rows = _flat(mask_rows, "mask_rows", torch.int32, ncols, dev)
-    token = lse = None
+        mp, ms, mr = mask.data_ptr(), mask.stride()[0], _flat(mask_rows, "mask_rows", i32, ncols, dev)
+    elif mask_rows is not None:
+        raise Q4KError(1, "mask_rows without a mask")
+    tp = sp = 0
     if pick:
-        token, lse = _new((ncols,), torch.int32, dev, stream), _new((ncols,), torch.float32, dev, stream)
-        a.token, a.lse = token.data_ptr(), lse.data_ptr()
-    _check(_call_on(dev, stream, lib().q4k_logits_process, ctypes.byref(a), ncols))
+        token, lse = _new(lg, (ncols,), i32, stream), _new(lg, (ncols,), None, stream)
+        tp, sp = token.data_ptr(), lse.data_ptr()
+    st = _call_on(dev, stream, lib().q4k_logits_process,
+                  _PACK_LOGITS.pack(lg.data_ptr(), o.data_ptr(), nvocab, lg.stride()[0], o.stride()[0], hp, lp, pp, hmax,
+                                    hs, bt, bv, bo, nb, mp, mr, ms, nm, tp, sp), ncols)
+    if st:
+        _check(st)
     return (out, token, lse) if pick else out
 
 

@@ -142,3 +142,12 @@ def test_python_wrappers_refuse_cpu_tensors(q4k):
         with pytest.raises(q4k.Q4KError) as e:
             call()
         assert e.value.status == EINVAL
+
+
+def test_packed_structs_are_the_structures(q4k):
+    """The wrappers' packed bytes and the ctypes structures lay the same fields at the same places."""
+    for pack, struct in ((q4k._PACK_LORA, q4k.LoraTask), (q4k._PACK_ROPE, q4k.RopeTensor), (q4k._PACK_LOGITS, q4k.LogitsArgs)):
+        assert pack.size == ctypes.sizeof(struct)
+        values = list(range(1, len(struct._fields_) + 1))
+        s = struct.from_buffer_copy(pack.pack(*values))
+        assert [getattr(s, f[0]) for f in struct._fields_] == values
