@@ -30,6 +30,7 @@ struct RopeParams {
     int ntensors, head_dim, n_rot, n_axes, order, layout, sect_sum;
     int sect[Q4K_MAX_ROPE_AXES];
     float scale;
+    int heads, lanes, heads_per_block;
 };
 
 template <typename T> __device__ __forceinline__ T from_f32(float v);
@@ -47,28 +48,36 @@ __device__ __forceinline__ int axis_of(const RopeParams &P, int i) {
     return a;
 }
 
-// One block per column: the column's cosines and sines go to shared memory
-// once and serve every head of every tensor.
+// Cosine and sine of pair i of column j, times the scale.
+__device__ __forceinline__ float2 turn_of(const RopeParams &P, int i, int64_t j) {
+    const double turns = static_cast<double>(P.pos[axis_of(P, i) * P.sp_axis + j]) * P.inv_freq[i] *
+                         0.31830988618379067154;  // 1/pi: half turns
+    const double r = turns - 2.0 * rint(0.5 * turns);
+    float s, c;
+    sincospif(static_cast<float>(r), &s, &c);
+    return make_float2(c * P.scale, s * P.scale);
+}
+
+#ifndef ROPE_COLS
+#define ROPE_COLS 592
+#endif
+constexpr int kThreads = 256;
+
+// Any sizes and strides: one block per column, one pair (or value behind the
+// pairs) at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) k_rope(const __grid_constant__ RopeParams P) {
+__global__ void __launch_bounds__(kThreads) k_rope(const __grid_constant__ RopeParams P) {
     __shared__ float2 cs[Q4K_MAX_ROPE_DIM / 2];
     const int64_t j = blockIdx.x;
     const int half = P.n_rot / 2;
-    for (int i = threadIdx.x; i < half; i += 256) {
-        const double turns = static_cast<double>(P.pos[axis_of(P, i) * P.sp_axis + j]) * P.inv_freq[i] *
-                             0.31830988618379067154;  // 1/pi: half turns
-        const double r = turns - 2.0 * rint(0.5 * turns);
-        float s, c;
-        sincospif(static_cast<float>(r), &s, &c);
-        cs[i] = make_float2(c * P.scale, s * P.scale);
-    }
+    for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = turn_of(P, i, j);
     __syncthreads();
     for (int k = 0; k < P.ntensors; ++k) {
         const RopeTensor &t = P.t[k];
         const float *x = t.x + j * t.sx_col;
         T *d = static_cast<T *>(t.dst) + j * t.sd_col;
         const int per = P.head_dim - half;  // pairs, then the values behind them
-        for (int w = threadIdx.x; w < t.heads * per; w += 256) {
+        for (int w = threadIdx.x; w < t.heads * per; w += kThreads) {
             const int h = w / per, i = w - h * per;
             const float *xh = x + h * t.sx_head;
             T *dh = d + h * t.sd_head;
@@ -83,6 +92,108 @@ __global__ void __launch_bounds__(256) k_rope(const __grid_constant__ RopeParams
             }
         }
     }
+}
+
+template <typename T> __device__ __forceinline__ void store4(T *d, const float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(d) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        T t[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(t);
+    }
+}
+
+// Heads of whole groups of four pairs (and of eight values behind them), all
+// 16-byte aligned. What has to move is x and dst once; the angles cost one
+// fp64 product and one sine per pair and column. A block takes a column and a
+// share of its heads (of all tensors, one after the other); a thread keeps one
+// group of four pairs, so its cosines and sines stay in registers, and walks
+// over the heads. Its first values are asked for before the angles are formed.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(kThreads) k_rope_vec(const __grid_constant__ RopeParams P) {
+    __shared__ float2 cs[Q4K_MAX_ROPE_DIM / 2];
+    const int64_t j = blockIdx.x;
+    const int half = P.n_rot / 2, groups = half / 4 + (P.head_dim - P.n_rot) / 8;
+    const int g = threadIdx.x & (P.lanes - 1), step = kThreads / P.lanes;  // lanes: groups, up to a power of two
+    const bool live = g < groups, pairs = g * 4 < half;
+    // the group's two runs of four values
+    const int lo = !pairs ? P.n_rot + (g - half / 4) * 8 : HALF ? g * 4 : g * 8;
+    const int hi = pairs && HALF ? lo + half : lo + 4;
+    int h = blockIdx.y * P.heads_per_block + threadIdx.x / P.lanes;
+    const int h1 = min(P.heads, static_cast<int>(blockIdx.y + 1) * P.heads_per_block);
+    auto tensor_of = [&](int &head) {
+        int k = 0;
+        while (head >= P.t[k].heads) head -= P.t[k++].heads;
+        return k;
+    };
+    float4 a, b;
+    auto load = [&](int head) {
+        const RopeTensor &t = P.t[tensor_of(head)];
+        const float *x = t.x + j * t.sx_col + head * t.sx_head;
+        a = *reinterpret_cast<const float4 *>(x + lo);
+        b = *reinterpret_cast<const float4 *>(x + hi);
+    };
+    if (live && h < h1) load(h);
+    for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = turn_of(P, i, j);
+    __syncthreads();
+    if (!live) return;
+    float c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        c[i] = pairs ? cs[g * 4 + i].x : 1.0f;
+        s[i] = pairs ? cs[g * 4 + i].y : 0.0f;
+    }
+    for (; h < h1; h += step) {
+        // values (a, b) of the four pairs: two runs, or neighbours
+        float xa[4] = {a.x, HALF ? a.y : a.z, HALF ? a.z : b.x, HALF ? a.w : b.z};
+        float xb[4] = {HALF ? b.x : a.y, HALF ? b.y : a.w, HALF ? b.z : b.y, b.w};
+        float ya[4], yb[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ya[i] = pairs ? fmaf(xa[i], c[i], -(xb[i] * s[i])) : xa[i];
+            yb[i] = pairs ? fmaf(xb[i], c[i], xa[i] * s[i]) : xb[i];
+        }
+        int head = h;
+        const RopeTensor &t = P.t[tensor_of(head)];
+        T *d = static_cast<T *>(t.dst) + j * t.sd_col + head * t.sd_head;
+        if (h + step < h1) load(h + step);
+        if (HALF) {
+            store4(d + lo, ya);
+            store4(d + hi, yb);
+        } else {
+            const float y0[4] = {ya[0], yb[0], ya[1], yb[1]}, y1[4] = {ya[2], yb[2], ya[3], yb[3]};
+            store4(d + lo, y0);
+            store4(d + hi, y1);
+        }
+    }
+}
+
+template <typename T> cudaError_t launch_rope(RopeParams &p, int ncols, cudaStream_t s) {
+    const int half = p.n_rot / 2, rest = p.head_dim - p.n_rot, groups = half / 4 + rest / 8;
+    bool vec = half % 4 == 0 && rest % 8 == 0 && groups > 0 && groups <= kThreads;
+    p.heads = 0;
+    for (int k = 0; k < p.ntensors; ++k) {
+        const RopeTensor &t = p.t[k];
+        p.heads += t.heads;
+        vec = vec && aligned_to(t.x, 16) && t.sx_col % 4 == 0 && t.sx_head % 4 == 0 && aligned_to(t.dst, 4 * sizeof(T)) &&
+              t.sd_col % 4 == 0 && t.sd_head % 4 == 0;
+    }
+    if (!vec) {
+        k_rope<T><<<ncols, kThreads, 0, s>>>(p);
+        return cudaGetLastError();
+    }
+    p.lanes = 1;
+    while (p.lanes < groups) p.lanes *= 2;
+    const int step = kThreads / p.lanes;
+    // a block takes all heads where there are columns for every SM several times over, else one step of them
+    p.heads_per_block = ncols >= ROPE_COLS ? p.heads : step;
+    while (p.heads / p.heads_per_block >= 65535) p.heads_per_block *= 2;  // (a grid's second dimension)
+    const dim3 grid(ncols, (p.heads + p.heads_per_block - 1) / p.heads_per_block);
+    if (p.layout == Q4K_ROPE_HALF)
+        k_rope_vec<T, true><<<grid, kThreads, 0, s>>>(p);
+    else
+        k_rope_vec<T, false><<<grid, kThreads, 0, s>>>(p);
+    return cudaGetLastError();
 }
 
 // heads x ncols runs of dim values: apart when one of the two strides steps over the other's whole span.
@@ -178,13 +289,9 @@ extern "C" int q4k_rope_multi(const q4k_rope_tensor *tensors, int ntensors, int 
     p.layout = layout;
     p.scale = scale;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (dst_type == Q4K_TYPE_F32)
-        k_rope<float><<<ncols, 256, 0, s>>>(p);
-    else if (dst_type == Q4K_TYPE_F16)
-        k_rope<__half><<<ncols, 256, 0, s>>>(p);
-    else
-        k_rope<__nv_bfloat16><<<ncols, 256, 0, s>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = dst_type == Q4K_TYPE_F32   ? launch_rope<float>(p, ncols, s)
+                          : dst_type == Q4K_TYPE_F16 ? launch_rope<__half>(p, ncols, s)
+                                                     : launch_rope<__nv_bfloat16>(p, ncols, s);
     if (e != cudaSuccess) return request_cuda_fail(e, "rope launch");
     return Q4K_OK;
 }
