@@ -22,7 +22,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
-import struct
+import sys
 from pathlib import Path
 from typing import Sequence
 
@@ -118,7 +118,7 @@ _SZ = ctypes.c_size_t
 def build() -> None:
     """Compile libq4k_gemv.so for sm_100a in-tree (nvcc cross-compiles without a GPU)."""
     import subprocess
-    subprocess.run(["make", "-C", str(HERE)], check=True)
+    subprocess.run(["make", f"PYTHON={sys.executable}", "-C", str(HERE)], check=True)
 
 
 def lib() -> ctypes.CDLL:
@@ -175,11 +175,11 @@ def lib() -> ctypes.CDLL:
             "q4k_ipc_close": (None, [_P]),
             "q4k_batch_ex_kernel": (_I, [TXP, _I, _I, _I]),
             "q4k_batch_persistent_kernel": (_I, [TP, _I, _I, _I]),
-            # (structs as void *: ctypes structures and packed bytes alike)
-            "q4k_lora_workspace_bytes": (_SZ, [_P, _I, _I]),
-            "q4k_lora_batch": (None, [_P, _I, _I, _P, _P, _SZ, _P]),
-            "q4k_rope_multi": (None, [_P, _I, _I, _I, _I, _P, _I64, _P, _P, _I, _I, _I, ctypes.c_float, _I, _P]),
-            "q4k_logits_process": (None, [_P, _I, _P]),
+            "q4k_lora_workspace_bytes": (_SZ, [ctypes.POINTER(LoraTask), _I, _I]),
+            "q4k_lora_batch": (None, [ctypes.POINTER(LoraTask), _I, _I, _P, _P, _SZ, _P]),
+            "q4k_rope_multi": (None, [ctypes.POINTER(RopeTensor), _I, _I, _I, _I, _P, _I64, _P, ctypes.POINTER(_I),
+                                      _I, _I, _I, ctypes.c_float, _I, _P]),
+            "q4k_logits_process": (None, [ctypes.POINTER(LogitsArgs), _I, _P]),
             "q4k_timeline_bytes": (_SZ, []),
             "q4k_timeline_read": (None, [_P, _SZ, ctypes.POINTER(_I)]),
             "q4k_timeline_reset": (None, []),
@@ -596,111 +596,36 @@ def debug_subblock_sums(W, yq, K: int, ws: Workspace | None = None, stream=None)
 # ---------------------------------------------------------------------------
 # what each request of a batch brings of its own: adapters, positions, controls
 # ---------------------------------------------------------------------------
-TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30  # Q4K_TYPE_*: ggml's type numbers
 ROPE_LAYOUTS = {"half": 0, "adjacent": 1}
 ROPE_ORDERS = {"blocks": 0, "interleaved": 1}
 
 
-# The structs above as the wrappers fill them: packed bytes cost a tenth of a
-# ctypes structure, and a small call's time is the host's.
-_PACK_LORA = struct.Struct("7Q9q3i4x")
-_PACK_ROPE = struct.Struct("2Q4qi4x")
-_PACK_LOGITS = struct.Struct("2Q3q3Q2q3Qq2Qqi4x2Q")
-_types: dict = {}  # torch dtype -> Q4K_TYPE_*
+_native_module = None
 
 
-def _type_of(dtype) -> int:
-    if not _types:
-        import torch
-        _types.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
-    t = _types.get(dtype)
-    if t is None:
-        raise Q4KError(1, f"type {dtype} is not float32, float16 or bfloat16")
-    return t
+def _native():
+    """The native front-end _q4k_torch, bound to the loaded library's entries (raises if it has not been built)."""
+    global _native_module
+    if _native_module is None:
+        import importlib.util
+        import torch  # noqa: F401  (its libraries are the module's)
+        path = HERE / "_q4k_torch.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it first (make -C {HERE})")
+        spec = importlib.util.spec_from_file_location("_q4k_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        L = lib()
+        mod.bind(Q4KError, *(ctypes.cast(getattr(L, name), _P).value
+                             for name in ("q4k_last_error", "q4k_lora_batch", "q4k_lora_workspace_bytes",
+                                          "q4k_rope_multi", "q4k_logits_process")))
+        _native_module = mod
+    return _native_module
 
 
-def _dense(t, name: str, ndim: int, dtype, device: int):
-    """t, checked: on CUDA device `device`, of `dtype` (None: any) and `ndim` dimensions, the last one contiguous."""
-    if t.dim() != ndim or t.get_device() != device or (dtype is not None and t.dtype != dtype):
-        raise Q4KError(1, f"{name}: {ndim}-d {dtype or 'tensor'} on cuda:{device} expected, got {tuple(t.shape)} "
-                          f"{t.dtype} on {t.device}")
-    if t.stride()[-1] != 1 and t.shape[-1] > 1:
-        raise Q4KError(1, f"{name}: the last dimension is not contiguous")
-    return t
-
-
-def _flat(t, name: str, dtype, n: int, device: int) -> int:
-    """Address of a contiguous 1-d tensor of n values (None: 0)."""
-    if t is None:
-        return 0
-    if t.get_device() != device or t.dtype != dtype or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
-        raise Q4KError(1, f"{name}: {n} contiguous values of {dtype} on cuda:{device} expected, got {tuple(t.shape)} "
-                          f"{t.dtype} on {t.device}")
-    return t.data_ptr()
-
-
-def _cuda_index(t, name: str) -> int:
-    if not t.is_cuda:
-        raise Q4KError(1, f"{name}: not a CUDA tensor (there is no CPU fallback)")
-    return t.get_device()
-
-
-def _new(like, shape, dtype, stream):
-    """An uninitialised tensor on like's device that belongs to the stream the call runs on."""
-    import torch
-    if stream is None:
-        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=like.device)
-    with torch.cuda.stream(stream):
-        return like.new_empty(shape, dtype=dtype)
-
-
-def _call_on(device: int, stream, fn, *args) -> int:
-    """fn(*args, stream) with the tensors' device current; stream None: that device's current one."""
-    import torch
-    s = torch._C._cuda_getCurrentRawStream(device) if stream is None else _stream(stream)
-    if device == torch.cuda.current_device():
-        return fn(*args, s)
-    with torch.cuda.device(device):
-        return fn(*args, s)
-
-
-def _lora_pack(x, A, B, base, ranks, scales, out, stream):
-    """One q4k_lora_task as bytes; returns (bytes, output, ncols, device index, type)."""
-    import torch
-    f32 = torch.float32
-    dev = _cuda_index(x, "x")
-    if x.dim() == 1:
-        x = x.unsqueeze(0)
-    ncols, K = _dense(x, "x", 2, f32, dev).shape
-    slots, rank, ka = _dense(A, "A", 3, None, dev).shape
-    sb, nrows, rb = _dense(B, "B", 3, A.dtype, dev).shape
-    if ka != K or sb != slots or rb != rank:
-        raise Q4KError(1, f"A {tuple(A.shape)} and B {tuple(B.shape)} do not fit x {tuple(x.shape)}")
-    if out is None:
-        out = _new(x, (ncols, nrows), None, stream)
-        o = out
-    else:
-        o = out.unsqueeze(0) if out.dim() == 1 else out
-        if _dense(o, "out", 2, f32, dev).shape != (ncols, nrows):
-            raise Q4KError(1, f"out {tuple(out.shape)}: ({ncols}, {nrows}) expected")
-    bp = bs = 0
-    if base is not None:
-        b = base.unsqueeze(0) if base.dim() == 1 else base
-        if _dense(b, "base", 2, f32, dev).shape != (ncols, nrows):
-            raise Q4KError(1, f"base {tuple(base.shape)}: ({ncols}, {nrows}) expected")
-        bp, bs = b.data_ptr(), b.stride()[0]
-    sa, sbs = A.stride(), B.stride()
-    kind = _type_of(A.dtype)
-    buf = _PACK_LORA.pack(x.data_ptr(), bp, o.data_ptr(), A.data_ptr(), B.data_ptr(),
-                          _flat(ranks, "ranks", torch.int32, slots, dev), _flat(scales, "scales", f32, slots, dev),
-                          K, nrows, x.stride()[0], bs, o.stride()[0], sa[0], sa[1], sbs[0], sbs[1], slots, rank, kind)
-    return buf, out, ncols, dev
-
-
-def _lora_pack_item(it: dict, stream):
-    return _lora_pack(it["x"], it["A"], it["B"], it.get("base"), it.get("ranks"), it.get("scales"), it.get("out"), stream)
+def _handle(stream):
+    """None (the tensors' device's current stream) or a stream's handle."""
+    return stream if stream is None or isinstance(stream, int) else stream.cuda_stream
 
 
 def make_lora_tasks(items: Sequence):
@@ -710,26 +635,7 @@ def make_lora_tasks(items: Sequence):
     int32) and scales (slots fp32).  The tensors must outlive the array."""
     if any(it.get("out") is None for it in items):
         raise Q4KError(1, "make_lora_tasks: an item has no out")
-    return (LoraTask * len(items)).from_buffer_copy(b"".join(_lora_pack_item(it, None)[0] for it in items))
-
-
-def _lora_call(tasks, n: int, ncols: int, ids, dev: int, ws, stream) -> None:
-    import torch
-    idp = _flat(ids, "ids", torch.int32, ncols, dev)
-    fn = lib().q4k_lora_batch
-    st = _call_on(dev, stream, fn, tasks, n, ncols, idp, ws.ptr if ws is not None else None,
-                  ws.nbytes if ws is not None else 0)
-    if st == 5:
-        need = int(lib().q4k_lora_workspace_bytes(tasks, n, ncols))
-        if ws is not None:
-            ws.ensure(need)
-            p = ws.ptr
-        else:  # scratch of this call's own, so calls on several streams or in several graphs share nothing
-            scratch = _new(ids, (need,), torch.uint8, stream)
-            p = scratch.data_ptr()
-        st = _call_on(dev, stream, fn, tasks, n, ncols, idp, p, need)
-    if st:
-        _check(st)
+    return (LoraTask * len(items)).from_buffer_copy(_native().lora_pack(items))
 
 
 def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
@@ -739,24 +645,13 @@ def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
     adapter, out[j] = base[j]).  tasks: dicts as for make_lora_tasks (out may be left
     out), returns the list of outputs; or its array, returns None."""
     if isinstance(tasks, ctypes.Array):
-        _lora_call(tasks, len(tasks), ids.shape[0], ids, _cuda_index(ids, "ids"), ws, stream)
-        return None
-    if len(tasks) == 0:
-        return []
-    got = [_lora_pack_item(it, stream) for it in tasks]
-    ncols, dev = got[0][2:]
-    for g in got:
-        if g[2] != ncols or g[3] != dev:
-            raise Q4KError(1, "the tasks' columns or devices differ")
-    _lora_call(b"".join([g[0] for g in got]), len(got), ncols, ids, dev, ws, stream)
-    return [g[1] for g in got]
+        return _native().lora_run(tasks, ids, ws, _handle(stream))
+    return _native().lora_batch(tasks, ids, ws, _handle(stream))
 
 
 def lora_add(x, A, B, ids, base=None, ranks=None, scales=None, out=None, ws: Workspace | None = None, stream=None):
     """lora_batch for one projection; returns (ncols, nrows) fp32."""
-    buf, out, ncols, dev = _lora_pack(x, A, B, base, ranks, scales, out, stream)
-    _lora_call(buf, 1, ncols, ids, dev, ws, stream)
-    return out
+    return _native().lora_add(x, A, B, ids, base, ranks, scales, out, ws, _handle(stream))
 
 
 def rope_inv_freq(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, factors=None, device=None):
@@ -778,46 +673,10 @@ def rope_multi(x, pos, inv_freq, sections, layout: str = "half", order: str = "b
     (i, i + n_rot/2), "adjacent" (2i, 2i+1); order: "blocks" or "interleaved" axes
     (include/q4k_gemv.h).  out: tensor(s) like x, x itself to turn in place, or None (new, of
     `dtype`: fp32, fp16 or bf16).  Returns out."""
-    import torch
-    single = not isinstance(x, (list, tuple))
-    xs = [x] if single else x
-    lay, order_id = ROPE_LAYOUTS.get(layout), ROPE_ORDERS.get(order)
-    if lay is None or order_id is None:
+    lay, turn = ROPE_LAYOUTS.get(layout), ROPE_ORDERS.get(order)
+    if lay is None or turn is None:
         raise Q4KError(1, f"layout {layout!r} / order {order!r}")
-    outs = [None] * len(xs) if out is None else [out] if single else list(out)
-    if not 1 <= len(xs) <= 4 or len(outs) != len(xs):
-        raise Q4KError(1, "1 to 4 tensors, and as many outputs")
-    f32 = torch.float32
-    dev = _cuda_index(xs[0], "x")
-    ncols, _, dim = _dense(xs[0], "x", 3, f32, dev).shape
-    if dtype is None:
-        dtype = outs[0].dtype if outs[0] is not None else f32
-    kind = _type_of(dtype)
-    packed = []
-    for i, v in enumerate(xs):
-        if i:
-            _dense(v, "x", 3, f32, dev)
-        c, heads, d = shape = v.shape
-        if c != ncols or d != dim:
-            raise Q4KError(1, f"x {tuple(shape)}: ({ncols}, heads, {dim}) expected")
-        o = outs[i]
-        if o is None:
-            o = outs[i] = _new(v, shape, dtype, stream)
-        elif _dense(o, "out", 3, dtype, dev).shape != shape:
-            raise Q4KError(1, f"out {tuple(o.shape)}: {tuple(shape)} expected")
-        sv, so = v.stride(), o.stride()
-        packed.append(_PACK_ROPE.pack(v.data_ptr(), o.data_ptr(), sv[0], sv[1], so[0], so[1], heads))
-    _dense(pos, "pos", 2, torch.int32, dev)
-    n = len(sections)
-    if pos.shape != (n, ncols):
-        raise Q4KError(1, f"pos {tuple(pos.shape)}: ({n}, {ncols}) expected")
-    half = inv_freq.shape[0]
-    st = _call_on(dev, stream, lib().q4k_rope_multi, b"".join(packed), len(xs), ncols, dim, 2 * half, pos.data_ptr(),
-                  pos.stride()[0], _flat(inv_freq, "inv_freq", torch.float64, half, dev), struct.pack(f"{n}i", *sections),
-                  n, order_id, lay, scale, kind)
-    if st:
-        _check(st)
-    return outs[0] if single else outs
+    return _native().rope(x, pos, inv_freq, sections, lay, turn, scale, dtype, out, _handle(stream))
 
 
 def logits_process(logits, history=None, history_len=None, penalties=None, bias_tokens=None, bias_values=None,
@@ -830,56 +689,8 @@ def logits_process(logits, history=None, history_len=None, penalties=None, bias_
     uint32, bit set = allowed, else -inf.  out may be logits itself.  Returns out; with
     pick=True (out, token, lse): the lowest index of the largest value (-1: nothing left) and
     log(sum(exp)) of every column."""
-    import torch
-    i32, f32 = torch.int32, torch.float32
-    dev = _cuda_index(logits, "logits")
-    lg = logits.unsqueeze(0) if logits.dim() == 1 else logits
-    ncols, nvocab = _dense(lg, "logits", 2, f32, dev).shape
-    if out is None:
-        out = _new(lg, logits.shape, None, stream)
-        o = out.unsqueeze(0) if out.dim() == 1 else out
-    else:
-        o = out.unsqueeze(0) if out.dim() == 1 else out
-        if _dense(o, "out", 2, f32, dev).shape != lg.shape:
-            raise Q4KError(1, f"out {tuple(out.shape)}: {tuple(logits.shape)} expected")
-    hp = lp = pp = hmax = hs = 0
-    if history is not None:
-        hrows, hmax = _dense(history, "history", 2, i32, dev).shape
-        if penalties is None or hrows != ncols:
-            raise Q4KError(1, f"history {tuple(history.shape)}: {ncols} rows, with penalties, expected")
-        if _dense(penalties, "penalties", 2, f32, dev).shape != (ncols, 3) or not penalties.is_contiguous():
-            raise Q4KError(1, f"penalties {tuple(penalties.shape)}: ({ncols}, 3) contiguous expected")
-        hp, lp, pp = history.data_ptr(), _flat(history_len, "history_len", i32, ncols, dev), penalties.data_ptr()
-        hs = history.stride()[0]
-    elif penalties is not None or history_len is not None:
-        raise Q4KError(1, "history and penalties go together")
-    bt = bv = bo = nb = 0
-    if bias_tokens is not None:
-        if bias_values is None or bias_offsets is None:
-            raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
-        nb = bias_tokens.shape[0]
-        bt, bv = _flat(bias_tokens, "bias_tokens", i32, nb, dev), _flat(bias_values, "bias_values", f32, nb, dev)
-        bo = _flat(bias_offsets, "bias_offsets", i32, ncols + 1, dev)
-    elif bias_values is not None or bias_offsets is not None:
-        raise Q4KError(1, "bias_tokens, bias_values and bias_offsets go together")
-    mp = mr = ms = nm = 0
-    if mask is not None:
-        nm, words = _dense(mask, "mask", 2, None, dev).shape
-        if mask.dtype not in (i32, torch.uint32) or words != (nvocab + 31) // 32:
-            raise Q4KError(1, f"mask {tuple(mask.shape)} {mask.dtype}: (masks, {(nvocab + 31) // 32}) int32 expected")
-        mp, ms, mr = mask.data_ptr(), mask.stride()[0], _flat(mask_rows, "mask_rows", i32, ncols, dev)
-    elif mask_rows is not None:
-        raise Q4KError(1, "mask_rows without a mask")
-    tp = sp = 0
-    if pick:
-        token, lse = _new(lg, (ncols,), i32, stream), _new(lg, (ncols,), None, stream)
-        tp, sp = token.data_ptr(), lse.data_ptr()
-    st = _call_on(dev, stream, lib().q4k_logits_process,
-                  _PACK_LOGITS.pack(lg.data_ptr(), o.data_ptr(), nvocab, lg.stride()[0], o.stride()[0], hp, lp, pp, hmax,
-                                    hs, bt, bv, bo, nb, mp, mr, ms, nm, tp, sp), ncols)
-    if st:
-        _check(st)
-    return (out, token, lse) if pick else out
+    return _native().logits(logits, history, history_len, penalties, bias_tokens, bias_values, bias_offsets, mask,
+                            mask_rows, out, pick, _handle(stream))
 
 
 # ---------------------------------------------------------------------------

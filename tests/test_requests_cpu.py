@@ -144,10 +144,13 @@ def test_python_wrappers_refuse_cpu_tensors(q4k):
         assert e.value.status == EINVAL
 
 
-def test_packed_structs_are_the_structures(q4k):
-    """The wrappers' packed bytes and the ctypes structures lay the same fields at the same places."""
-    for pack, struct in ((q4k._PACK_LORA, q4k.LoraTask), (q4k._PACK_ROPE, q4k.RopeTensor), (q4k._PACK_LOGITS, q4k.LogitsArgs)):
-        assert pack.size == ctypes.sizeof(struct)
-        values = list(range(1, len(struct._fields_) + 1))
-        s = struct.from_buffer_copy(pack.pack(*values))
-        assert [getattr(s, f[0]) for f in struct._fields_] == values
+def test_structures_match_the_header(q4k):
+    """The ctypes structures are as large as the native front-end's C structs (one task's bytes)."""
+    import torch
+    assert q4k._native().lora_pack([]) == b""
+    assert ctypes.sizeof(q4k.LoraTask) == 7 * 8 + 9 * 8 + 4 * 4
+    assert ctypes.sizeof(q4k.RopeTensor) == 2 * 8 + 4 * 8 + 8
+    assert ctypes.sizeof(q4k.LogitsArgs) == 20 * 8
+    with pytest.raises(q4k.Q4KError):
+        q4k.lora_batch([dict(x=torch.zeros(1, 8))], torch.zeros(1, dtype=torch.int32))
+    assert q4k.lora_batch([], torch.zeros(1, dtype=torch.int32)) == []
