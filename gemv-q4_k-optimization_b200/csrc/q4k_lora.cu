@@ -94,18 +94,21 @@ template <typename T, int V> __device__ __forceinline__ Chunk<T, V> zero_chunk()
     for (int e = 0; e < V; ++e) c.v[e] = T(0.0f);
     return c;
 }
-// Values [0, n) of a row at p, n >= 1; the rest is zero and not read.
+// Values [0, n) of a row at p, n >= 1; the rest is zero and not read. The ends
+// of rows go out of line: inlined at every load they made the code several
+// times as long, and a short call waits for its instructions.
+template <typename T, int V> __device__ __noinline__ Chunk<T, V> load_end(const T *p, int n) {
+    Chunk<T, V> c = zero_chunk<T, V>();
+#pragma unroll
+    for (int e = 0; e < V - 1; ++e)
+        if (e < n) c.v[e] = p[e];
+    return c;
+}
 template <typename T, int V> __device__ __forceinline__ Chunk<T, V> load_chunk(const T *p, int n) {
     if constexpr (V > 1) {
-        if (n >= V) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
-            return *reinterpret_cast<const Chunk<T, V> *>(&raw);
-        }
-        Chunk<T, V> c = zero_chunk<T, V>();
-#pragma unroll
-        for (int e = 0; e < V - 1; ++e)
-            if (e < n) c.v[e] = p[e];
-        return c;
+        if (n < V) return load_end<T, V>(p, n);
+        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
+        return *reinterpret_cast<const Chunk<T, V> *>(&raw);
     } else {
         Chunk<T, V> c;
         c.v[0] = __ldg(p);
@@ -168,7 +171,8 @@ __device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, uint
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int c = c0 + i * L * VB;
-            wb[i] = n < n1 && c < r ? load_chunk<T, VB>(B + n * t.sb_row + c, r - c) : zero_chunk<T, VB>();
+            // (a chunk that begins below r is read as far as the row has room; values behind r are not used)
+            wb[i] = n < n1 && c < r ? load_chunk<T, VB>(B + n * t.sb_row + c, t.rank - c) : zero_chunk<T, VB>();
         }
     };
     auto ask_base = [&]() {
