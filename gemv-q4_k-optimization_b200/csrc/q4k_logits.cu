@@ -44,7 +44,10 @@ struct LogitsParams {
 constexpr int kThreads = LG_T;
 constexpr int kQuads = LG_Q;                      // groups of 4 tokens per thread and chunk (at most 8)
 constexpr int kChunk = kThreads * kQuads * 4;     // tokens in flight per CTA
-constexpr int kSegment = 65536;                   // tokens whose listed places are held at a time
+#ifndef LG_SEG
+#define LG_SEG 65536
+#endif
+constexpr int kSegment = LG_SEG;                   // tokens whose listed places are held at a time
 constexpr int kMinSlots = 256, kMaxSlots = 4096;  // listed tokens with room for their count and bias sum
 constexpr int kAhead = 4;                         // list entries per thread in registers
 constexpr float kLog2e = 1.4426950408889634f;
@@ -75,17 +78,18 @@ __device__ __forceinline__ Stat shfl_xor(const Stat &v, int o) {
 }
 
 // The listed tokens of one segment of a CTA's slice: a bit per token, the
-// number of bits before each word, and a slot {token, count, bias sum} per
-// listed token, found by its rank among them.
+// number of bits before each word, and a slot {token, count, number of biases,
+// bias sum} per listed token, found by its rank among them.
 struct Lists {
     uint32_t touched[kSegment / 32];
     uint16_t before[kSegment / 32];
     uint32_t sums[kThreads / 32];
-    int token[kMaxSlots];  // `slots` of them, then as many counts and bias sums: the launch sizes the memory
+    int repeats;           // whether a token has several biases
+    int token[kMaxSlots];  // `slots` of them, then as many of the others: the launch sizes the memory
 };
 
 // What a CTA knows of its column's lists: history entries [0, nh), bias entries
-// [b0, b1), the first of them in registers.
+// [b0, b1), each thread's first ones in registers.
 struct Column {
     const int32_t *history;
     int nh, b0, b1;
@@ -93,30 +97,14 @@ struct Column {
     float bval[kAhead];
 };
 
-// f(token) for every history entry, by all threads; g(token, value, entries) for
-// the bias entries by the last warp, 32 entries in list order at a time.
+// f(token) for every history entry, g(token, value) for every bias entry, in no order.
 template <typename F, typename G>
 __device__ __forceinline__ void for_lists(const LogitsParams &P, const Column &C, F f, G g) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (tid / 32 == kThreads / 32 - 1) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (C.b0 + i * 32 < C.b1) g(C.btok[i], C.bval[i]);
-        for (int e0 = C.b0 + kAhead * 32; e0 < C.b1; e0 += kAhead * 32) {
-            int tok[kAhead];
-            float val[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int e = e0 + lane + i * 32;
-                tok[i] = e < C.b1 ? P.bias_tokens[e] : -1;
-                val[i] = e < C.b1 ? P.bias_values[e] : 0.0f;
-            }
-#pragma unroll 1
-            for (int i = 0; i < kAhead; ++i) g(tok[i], val[i]);
-        }
-    }
+    const int tid = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) f(C.htok[i]);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) g(C.btok[i], C.bval[i]);
     for (int e0 = kAhead * kThreads + tid; e0 < C.nh; e0 += kAhead * kThreads) {
         int tok[kAhead];
 #pragma unroll
@@ -124,20 +112,24 @@ __device__ __forceinline__ void for_lists(const LogitsParams &P, const Column &C
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) f(tok[i]);
     }
+    for (int e = C.b0 + kAhead * kThreads + tid; e < C.b1; e += kThreads) g(P.bias_tokens[e], P.bias_values[e]);
 }
 
 // Finds the listed ones of the tokens [base, base + n): counts (integer
-// atomics: any order gives the same) and bias sums (one warp, in list order).
-// Returns how many there are; with more than `slots` nothing is summed.
+// atomics: any order gives the same) and bias sums (in list order where a token
+// has several). Returns how many there are; with more than `slots` nothing is
+// summed.
 __device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C, Lists &S, int base, int n) {
     const int tid = threadIdx.x, lane = tid & 31, words = (n + 31) / 32, slots = P.slots;
-    int *count = S.token + slots;
-    float *bias = reinterpret_cast<float *>(count + slots);
+    int *count = S.token + slots, *biases = count + slots;
+    float *bias = reinterpret_cast<float *>(biases + slots);
     for (int i = tid; i < words; i += kThreads) S.touched[i] = 0u;
     for (int i = tid; i < slots; i += kThreads) {
         count[i] = 0;
+        biases[i] = 0;
         bias[i] = 0.0f;
     }
+    if (tid == 0) S.repeats = 0;
     __syncthreads();
     auto in = [&](int tok) { return tok >= 0 && tok >= base && tok - base < n; };
     auto mark = [&](int tok) {
@@ -170,32 +162,44 @@ __device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C
     __syncthreads();
     if (static_cast<int>(total) > slots) return static_cast<int>(total);
     auto slot = [&](int tok) {
-        if (!in(tok)) return -1;
-        const int i = tok - base, k = S.before[i >> 5] + __popc(S.touched[i >> 5] & ((1u << (i & 31)) - 1u));
-        S.token[k] = tok;
-        return k;
+        const int i = tok - base;
+        return S.before[i >> 5] + __popc(S.touched[i >> 5] & ((1u << (i & 31)) - 1u));
     };
     for_lists(
         P, C,
         [&](int tok) {
+            if (!in(tok)) return;
             const int i = slot(tok);
-            if (i >= 0) atomicAdd(&count[i], 1);
+            S.token[i] = tok;
+            atomicAdd(&count[i], 1);
         },
         [&](int tok, float val) {
+            if (!in(tok)) return;
             const int i = slot(tok);
-            if (!__any_sync(0xffffffffu, i >= 0)) return;
-            const unsigned same = __match_any_sync(0xffffffffu, i >= 0 ? i : -1 - lane);
-            if (__any_sync(0xffffffffu, __popc(same) > 1)) {
-                for (int q = 0; q < 32; ++q) {  // a token twice: one entry after the other
-                    if (lane == q && i >= 0) bias[i] += val;
-                    __syncwarp();
-                }
-            } else if (i >= 0) {
-                bias[i] += val;
-            }
-            __syncwarp();
+            S.token[i] = tok;
+            // (a token's only bias stays as it is stored here; of several, the sum below is formed anew)
+            if (atomicAdd(&biases[i], 1) > 0)
+                S.repeats = 1;
+            else
+                bias[i] = 0.0f + val;
         });
     __syncthreads();
+    if (S.repeats && tid < 32) {  // one warp adds up the tokens with several biases, in list order
+        for (int i = lane; i < static_cast<int>(total); i += 32)
+            if (biases[i] > 1) bias[i] = 0.0f;
+        __syncwarp();
+        for (int e0 = C.b0; e0 < C.b1; e0 += 32) {
+            const int tok = e0 + lane < C.b1 ? P.bias_tokens[e0 + lane] : -1;
+            const float val = e0 + lane < C.b1 ? P.bias_values[e0 + lane] : 0.0f;
+            const int i = in(tok) ? slot(tok) : -1;
+            unsigned todo = __ballot_sync(0xffffffffu, i >= 0 && biases[max(i, 0)] > 1);
+            for (; todo != 0; todo &= todo - 1) {
+                if (lane == __ffs(todo) - 1) bias[i] += val;
+                __syncwarp();
+            }
+        }
+    }
+    if (S.repeats) __syncthreads();
     return static_cast<int>(total);
 }
 
@@ -268,10 +272,9 @@ __global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constan
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
         C.htok[i] = tid + i * kThreads < C.nh ? C.history[tid + i * kThreads] : -1;
-        const int e = C.b0 + lane + i * 32;
-        const bool mine = warp == kThreads / 32 - 1 && e < C.b1;
-        C.btok[i] = mine ? P.bias_tokens[e] : -1;
-        C.bval[i] = mine ? P.bias_values[e] : 0.0f;
+        const int e = C.b0 + tid + i * kThreads;
+        C.btok[i] = e < C.b1 ? P.bias_tokens[e] : -1;
+        C.bval[i] = e < C.b1 ? P.bias_values[e] : 0.0f;
     }
     Stat st = {-INFINITY, 0.0f, INT_MAX};
     float4 z[kQuads];
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constan
                 const int v = S.token[i], c = S.token[P.slots + i];
                 float y = -INFINITY;
                 if (mask == nullptr || (mask[v >> 5] >> (v & 31) & 1u)) {
-                    y = __fadd_rn(l[v], __int_as_float(S.token[2 * P.slots + i]));
+                    y = __fadd_rn(l[v], __int_as_float(S.token[3 * P.slots + i]));
                     if (c > 0) {
                         y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
                         y = __fsub_rn(y, __fadd_rn(__fmul_rn(static_cast<float>(c), freq), pres));
@@ -416,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constan
     }
 }
 
-size_t list_bytes(int slots) { return offsetof(Lists, token) + static_cast<size_t>(slots) * 12; }
+size_t list_bytes(int slots) { return offsetof(Lists, token) + static_cast<size_t>(slots) * 16; }
 
 cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     const bool v4 = p.nvocab >= 16 && reinterpret_cast<uintptr_t>(p.logits) / 4 % 4 == reinterpret_cast<uintptr_t>(p.dst) / 4 % 4 &&
@@ -435,9 +438,9 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
         }
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    // two CTAs for every SM if the vocabulary has a chunk for each
+    // eight CTAs for every SM (four are resident: the rest evens out their ends) if the vocabulary has a chunk for each
     int nc = 1;
-    while (nc < 16 && nc * kChunk < p.nvocab && (LG_NC ? nc < LG_NC : nc * static_cast<int64_t>(ncols) < 296)) nc *= 2;
+    while (nc < 16 && nc * kChunk < p.nvocab && (LG_NC ? nc < LG_NC : nc * static_cast<int64_t>(ncols) < 1184)) nc *= 2;
     // slots for a column's whole history and its likely biases (their number per column is known to the device
     // alone); a CTA whose tokens need more takes them in smaller segments
     const int64_t listed = p.max_history + (p.bias_tokens != nullptr ? 2 * static_cast<int64_t>(p.n_bias) / ncols + 64 : 0);
