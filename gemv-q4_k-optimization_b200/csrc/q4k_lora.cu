@@ -39,6 +39,7 @@ struct LoraParams {
     const int32_t *ids;
     int ntasks, ncols;
     // many columns only: workspace and splits
+    int *status;  // the workspace's status word
     int *ntiles;
     LoraTile *tiles;
     int *order;   // columns sorted by adapter
@@ -498,7 +499,10 @@ __global__ void __launch_bounds__(1024) k_lora_plan(const __grid_constant__ Lora
         at[b] = first;
         for (int i = 0; i < cols; i += kTileCols)
             P.tiles[tile++] = {b < P.max_slots ? b : -1, first + i, min(kTileCols, cols - i)};
-        if (b == bins - 1) *P.ntiles = tile;
+        if (b == bins - 1) {
+            *P.ntiles = tile;
+            *P.status = Q4K_OK;
+        }
     };
     if (tid < bins) list(tid, mine, upto[0] - c[0], upto[1] - c[1]);
     if (tid == 1023 && bins == 1025) list(1024, bin[1024], upto[0], upto[1]);
@@ -653,22 +657,63 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
     cluster.sync();  // no CTA leaves while another may still read its part
 }
 
-// dst of a tile's columns for a range of rows. Eight warps: 16 columns each, two
-// row groups. The pieces of u lie in shared memory; B comes through a ring of
-// stages of 64 rows x 64 ranks (32 in fp32, to fit beside the u of 512 ranks),
-// read once per CTA. A block is 16 columns x 32 rows; its rows are dealt
-// to the MMAs' columns so that a lane ends with eight consecutive rows of two
-// columns: base (asked for one block ahead) and dst move in 16-byte accesses.
-template <typename T> struct RowStage {
-    static constexpr int kK = sizeof(T) == 2 ? 64 : 32;  // ranks
-    static constexpr int kPitch = kK + 8;                // values between rows (rows meet in few banks)
-    static constexpr int kValues = 64 * kPitch;
-};
+// ---- expand: 5th-generation tensor cores ------------------------------------------
+// dst of a tile's columns for a range of rows, in tiles of 128 rows: D (128 rows
+// x 64 columns, fp32 in tensor memory) = pieces of B (128 x 64 ranks, shared
+// memory) x pieces of u (64 columns x 64 ranks). One thread issues the MMAs;
+// afterwards a lane of tensor memory is a row, so a warp reads base and writes
+// dst for 32 consecutive rows of a column at a time, whatever their alignment.
+// Operands lie K-major in rows of 128 bytes, 16-byte units exchanged within a
+// row by its index modulo 8 (the 128-byte swizzle).
+constexpr int kRows = 128;                     // rows of a tile
+constexpr int kChunkK = 64;                    // ranks of a chunk: one swizzled row of bf16
+constexpr int kUBytes = kTileCols * 128;       // one piece of u's chunk
+constexpr int kBBytes = kRows * 128;           // one piece of B's chunk
+constexpr int kTmemCols = 64;
+template <typename T> constexpr size_t kExpandSmem = 3 * kUBytes + Weight<T>::kPieces * kBBytes + 1024;  // (+ alignment)
 
-template <typename T, bool VB, bool VY>
-__global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ LoraParams P) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    constexpr int kK = RowStage<T>::kK, kPitch = RowStage<T>::kPitch, kValues = RowStage<T>::kValues;
+__device__ __forceinline__ uint32_t swizzled(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
+// Shared-memory operand descriptor: K-major, 128-byte swizzle, groups of eight rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
+           uint64_t(2) << 61;
+}
+// fp32 += bf16 x bf16, both operands K-major, M = 128, N = 64.
+constexpr uint32_t kMmaShape = 1u << 4 | 1u << 7 | 1u << 10 | (kTileCols / 8) << 17 | (kRows / 16) << 24;
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint64_t a, uint64_t b, bool add) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b),
+        "r"(kMmaShape), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// 16 columns of this warp's 32 lanes.
+__device__ __forceinline__ void load_tmem(uint32_t (&v)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr)
+        : "memory");
+}
+// Waits for a phase of the barrier, at most two seconds.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t until = globaltimer_ns() + 2000000000ull;
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer_ns() > until) return false;
+    return true;
+}
+
+template <typename T, bool VB>
+__global__ void __launch_bounds__(256, 3) k_lora_expand(const __grid_constant__ LoraParams P) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ struct {
+        const float *base;
+        float *dst;
+    } col[kTileCols];
+    __shared__ __align__(8) uint64_t done;  // the MMAs of a chunk
+    __shared__ uint32_t tmem;
     pdl_launch_dependents();
     pdl_wait();
     if (static_cast<int>(blockIdx.x) >= *P.ntiles) return;
@@ -677,7 +722,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ 
     const int n0 = blockIdx.y * P.rows_per_cta, n1 = min(t.nrows, n0 + P.rows_per_cta);
     if (n0 >= n1) return;
     const int a = slot_of(t, tile.slot), r = a < 0 ? 0 : rank_of(t, a);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (r == 0) {  // nothing to add
         for (int i = warp; i < tile.count; i += 8) {
             const int64_t j = P.order[tile.first + i];
@@ -685,125 +730,123 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand(const __grid_constant__ 
         }
         return;
     }
-    T *ring = reinterpret_cast<T *>(smem_raw);
-    const int chunks = (r + kK - 1) / kK, rp = chunks * kK, pitch = rp + 8;
-    uint16_t *up = reinterpret_cast<uint16_t *>(ring + kRing * kValues);  // [piece][column][pitch]
+    constexpr int N = Weight<T>::kPieces;
+    uint8_t *us = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *bs = us + 3 * kUBytes;
+    if (tid < tile.count) {
+        const int64_t j = P.order[tile.first + tid];
+        col[tid] = {t.base != nullptr ? t.base + j * t.sbase : nullptr, t.dst + j * t.sdst};
+    }
+    __syncwarp();
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem)), "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if (lane == 0) {
+            mbar_init(smem_addr(&done), 1);
+            mbar_fence_init();
+        }
+    }
     const T *B = static_cast<const T *>(t.B) + a * t.sb_slot;
-    const int stages = (n1 - n0 + 63) / 64 * chunks;
-    auto fill = [&](int s) {
-        if (s < stages) {
-            T *to = ring + (s % kRing) * kValues;
-            const int k0 = s % chunks * kK, row0 = n0 + s / chunks * 64;
-            if constexpr (VB) {
-                constexpr int E = 16 / sizeof(T), C = kK / E;  // values per copy, copies per row
+    const int chunks = (r + kChunkK - 1) / kChunkK, tiles = (n1 - n0 + kRows - 1) / kRows;
+    // chunk c of u (columns behind the tile's: zeros) and of the rows of tile i of B; zeros behind the rank and the rows
+    auto fill_u = [&](int c) {
+        for (int i = tid; i < 3 * kTileCols * 8; i += 256) {
+            const int unit = i & 7, row = (i >> 3) & (kTileCols - 1), piece = i / (8 * kTileCols), k = c * kChunkK + unit * 8;
+            const bool some = row < tile.count && k < r;
+            const uint16_t *u = some ? P.u + (static_cast<int64_t>(piece) * P.ncols + tile.first + row) * P.u_cols + t.u_off + k : P.u;
+            cp_async16(us + piece * kUBytes + swizzled(row, unit), u, some ? 16 : 0);
+        }
+    };
+    auto fill_b = [&](int i, int c) {
+        const int row0 = n0 + i * kRows;
 #pragma unroll
-                for (int i = tid; i < 64 * C; i += 256) {
-                    const int row = i / C, k = (i - row * C) * E, left = row0 + row < n1 ? min(E, r - k0 - k) : 0;
-                    const bool some = left > 0;
-                    cp_async16(to + row * kPitch + k, some ? B + (row0 + row) * t.sb_row + k0 + k : B,
-                               some ? left * static_cast<int>(sizeof(T)) : 0);
-                }
+        for (int e = 0; e < kRows * 8 / 256; ++e) {
+            const int unit = tid & 7, row = (tid >> 3) + e * 32, k = c * kChunkK + unit * 8;
+            const int left = row0 + row < n1 ? r - k : 0;
+            const T *from = B + (row0 + row) * t.sb_row + k;
+            if constexpr (VB && N == 1) {
+                cp_async16(bs + swizzled(row, unit), left > 0 ? from : B, left > 0 ? min(left, 8) * 2 : 0);
             } else {
-                for (int i = tid; i < 64 * kK; i += 256) {
-                    const int row = i / kK, k = i % kK;
-                    to[row * kPitch + k] = row0 + row < n1 && k0 + k < r ? B[(row0 + row) * t.sb_row + k0 + k] : T(0.0f);
-                }
+                uint32_t q[N][4];
+                weights(load_eight<T, VB>(from, left), q);
+#pragma unroll
+                for (int p = 0; p < N; ++p)
+                    *reinterpret_cast<uint4 *>(bs + p * kBBytes + swizzled(row, unit)) = make_uint4(q[p][0], q[p][1], q[p][2], q[p][3]);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // the pieces of u come with the first stage (zeros behind the rank)
-    for (int i = tid; i < 3 * tile.count * (rp / 8); i += 256) {
-        const int k = i % (rp / 8) * 8, pc = i / (rp / 8), piece = pc / tile.count, col = pc - piece * tile.count;
-        const uint16_t *u = P.u + (static_cast<int64_t>(piece) * P.ncols + tile.first + col) * P.u_cols + t.u_off;
-        cp_async16(up + (piece * kTileCols + col) * pitch + k, k < r ? u + k : u, k < r ? 16 : 0);
-    }
+    fill_u(0);
+    fill_b(0, 0);
+    bool bad = false;
+    uint32_t parity = 0;
+    for (int s = 0, i = 0, c = 0; i < tiles; ++s) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        // the operands have come, and (at first) the allocation; the tile before has been read out of tensor memory
+        if (__syncthreads_or(bad)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem;
+        if (tid == 0) {
+            bool add = c > 0;
 #pragma unroll
-    for (int i = 0; i < kRing - 1; ++i) fill(i);
-
-    const int m0 = (warp & 3) * 16;
-    const bool busy = m0 < tile.count;
-    const float *base[2];
-    float *dst[2];
+            for (int order = 2; order >= 0; --order)  // small products first
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int i = m0 + g + 8 * h;
-        const int64_t j = i < tile.count ? P.order[tile.first + i] : -1;
-        base[h] = j >= 0 && t.base != nullptr ? t.base + j * t.sbase : nullptr;
-        dst[h] = j >= 0 ? t.dst + j * t.sdst : nullptr;
-    }
-    int n = n0 + (warp >> 2) * 32 + 8 * q;  // the lane's first row of the block
-    auto load_base = [&](Eight<float> (&y)[2], int row) {
+                for (int p = 0; p < N; ++p)
+                    if (p <= order)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) y[h] = load_eight<float, VY>(base[h] + row, base[h] != nullptr ? n1 - row : 0);
-    };
-    Eight<float> y[2];
-    load_base(y, n);
-    float sum[4][4] = {};
-    for (int s = 0, c = 0; s < stages; ++s, c = c + 1 == chunks ? 0 : c + 1) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-        __syncthreads();  // stage s (and at first u) has come, and stage s - 1 may be written again
-        fill(s + kRing - 1);
-        if (!busy) continue;
-        const T *w = ring + (s % kRing) * kValues + (warp >> 2) * 32 * kPitch;
-        Eight<float> next[2];
-        if (c + 1 == chunks) load_base(next, n + 64);
-#pragma unroll
-        for (int k = 0; k < kK / 32; ++k) {
-            if (c * kK + k * 32 >= r) break;
-            uint32_t ua[2][3][4];
-#pragma unroll
-            for (int i = 0; i < 3; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // (rows behind the tile's columns hold anything: an MMA keeps rows apart)
-                    const uint4 v = *reinterpret_cast<const uint4 *>(up + (i * kTileCols + m0 + g + 8 * h) * pitch + c * kK +
-                                                                     k * 32 + 8 * q);
-                    ua[0][i][h] = v.x, ua[0][i][2 + h] = v.y, ua[1][i][h] = v.z, ua[1][i][2 + h] = v.w;
-                }
-            float acc[4][4];
-            products<T>(acc, ua, [&](int b) {
-                return load_eight_smem(w + (8 * (g >> 1) + 2 * b + (g & 1)) * kPitch + k * 32 + 8 * q);
-            });
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[b][e] += acc[b][e];
+                        for (int k = 0; k < kChunkK / 16; ++k) {
+                            mma_tmem(d, operand(smem_addr(bs) + p * kBBytes) + 2 * k,
+                                     operand(smem_addr(us) + (order - p) * kUBytes) + 2 * k, add);
+                            add = true;
+                        }
+            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(&done))
+                         : "memory");
         }
-        if (c + 1 < chunks) continue;
+        const bool last = c + 1 == chunks;
+        const int n = n0 + i * kRows + (warp & 3) * 32 + lane, c0 = warp / 4 * 32;
+        float y[16];
+        auto ask = [&](int from) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float *b = from + e < tile.count ? col[from + e].base : nullptr;
+                y[e] = b != nullptr && n < n1 ? b[n] : 0.0f;
+            }
+        };
+        if (last) ask(c0);
+        bad = __any_sync(0xffffffffu, !wait_bounded(smem_addr(&done), parity));  // (a warp leaves as one)
+        parity ^= 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        c = last ? 0 : c + 1;
+        i += last;
+        if (i < tiles && !bad) {  // (the MMAs are through with the operands)
+            if (chunks > 1) fill_u(c);
+            fill_b(i, c);
+        }
+        if (!last || bad) continue;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            uint32_t v[16];
+            __syncwarp();
+            load_tmem(v, d + ((warp & 3) * 32 << 16) + c0 + 16 * h);
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    y[h].v[2 * b + e] += sum[b][2 * h + e];
-                    sum[b][2 * h + e] = 0.0f;
-                }
-            if (dst[h] == nullptr) continue;
-            float *d = dst[h] + n;
-            if (VY && n + 8 <= n1) {
-                reinterpret_cast<float4 *>(d)[0] = reinterpret_cast<float4 *>(&y[h])[0];
-                reinterpret_cast<float4 *>(d)[1] = reinterpret_cast<float4 *>(&y[h])[1];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (n + e < n1) d[e] = y[h].v[e];
-            }
+            for (int e = 0; e < 16; ++e)
+                if (c0 + 16 * h + e < tile.count && n < n1) col[c0 + 16 * h + e].dst[n] = y[e] + __uint_as_float(v[e]);
+            if (h == 0) ask(c0 + 16);
         }
-        y[0] = next[0];
-        y[1] = next[1];
-        n += 64;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (bad) st_relaxed_gpu(P.status, Q4K_ETIMEOUT);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     }
 }
 
 template <typename T> constexpr size_t kShrinkSmem = kRing * kShrinkStage<T>;
-template <typename T> size_t expand_smem(int rank) {
-    constexpr int kK = RowStage<T>::kK;
-    return static_cast<size_t>(kRing) * RowStage<T>::kValues * sizeof(T) +
-           static_cast<size_t>(3) * kTileCols * ((rank + kK - 1) / kK * kK + 8) * 2;
-}
-
 // A launch that may begin while the one before it ends (its kernel waits for it).
 template <typename K>
 cudaError_t launch_next(K *fn, dim3 grid, int cluster_y, int threads, size_t smem, const LoraParams &p, cudaStream_t s) {
@@ -828,22 +871,20 @@ cudaError_t launch_next(K *fn, dim3 grid, int cluster_y, int threads, size_t sme
 int most_tiles(int ncols, int max_slots) { return ncols / kTileCols + (ncols < max_slots + 1 ? ncols : max_slots + 1); }
 
 template <typename T>
-cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool vy, int rank, cudaStream_t s) {
+cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, cudaStream_t s) {
     auto *shrink = vx ? va ? k_lora_shrink<T, true, true> : k_lora_shrink<T, true, false>
                       : va ? k_lora_shrink<T, false, true> : k_lora_shrink<T, false, false>;
-    auto *expand = vb ? vy ? k_lora_expand<T, true, true> : k_lora_expand<T, true, false>
-                      : vy ? k_lora_expand<T, false, true> : k_lora_expand<T, false, false>;
+    auto *expand = vb ? k_lora_expand<T, true> : k_lora_expand<T, false>;
     static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        const int ss = static_cast<int>(kShrinkSmem<T>), es = static_cast<int>(expand_smem<T>(Q4K_MAX_LORA_RANK));
+        const int ss = static_cast<int>(kShrinkSmem<T>), es = static_cast<int>(kExpandSmem<T>);
         for (auto *f : {k_lora_shrink<T, true, true>, k_lora_shrink<T, true, false>, k_lora_shrink<T, false, true>,
                         k_lora_shrink<T, false, false>})
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ss)) != cudaSuccess) return e;
-        for (auto *f : {k_lora_expand<T, true, true>, k_lora_expand<T, true, false>, k_lora_expand<T, false, true>,
-                        k_lora_expand<T, false, false>})
+        for (auto *f : {k_lora_expand<T, true>, k_lora_expand<T, false>})
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, es)) != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
@@ -860,7 +901,7 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, bool 
         if (e != cudaSuccess) return e;
     }
     return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 0, 256,
-                       expand_smem<T>(rank), p, s);
+                       kExpandSmem<T>, p, s);
 }
 
 // Whether every run of 8 values of every row is 16-byte aligned.
@@ -870,17 +911,16 @@ bool rows_aligned(const void *p, int64_t slot, int64_t row, int esz) {
 
 template <typename T> cudaError_t launch_lora(const LoraParams &p, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    bool va = true, vb = true, vx = true, vy = true;
+    bool va = true, vb = true, vx = true;
     int rank = 0;
     for (int i = 0; i < p.ntasks; ++i) {
         const LoraTask &t = p.task[i];
         va = va && rows_aligned(t.A, t.sa_slot, t.sa_row, sizeof(T));
         vb = vb && rows_aligned(t.B, t.sb_slot, t.sb_row, sizeof(T));
         vx = vx && rows_aligned(t.x, 0, t.sx, 4);
-        vy = vy && rows_aligned(t.dst, 0, t.sdst, 4) && rows_aligned(t.base, 0, t.base != nullptr ? t.sbase : 0, 4);
         rank = std::max(rank, t.rank);
     }
-    if (p.ncols > kClusterCols) return launch_grouped<T>(p, vx, va, vb, vy, rank, s);
+    if (p.ncols > kClusterCols) return launch_grouped<T>(p, vx, va, vb, s);
     const int n = p.ntasks;
     return va ? vb ? launch_cluster<T, V, V>(p, n, rank, s) : launch_cluster<T, V, 1>(p, n, rank, s)
               : vb ? launch_cluster<T, 1, V>(p, n, rank, s) : launch_cluster<T, 1, 1>(p, n, rank, s);
@@ -963,7 +1003,10 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
     return Q4K_OK;
 }
 
-// Workspace of the many-column path: number of tiles, tiles, order, u.
+#ifndef LORA_ROWS
+#define LORA_ROWS 512
+#endif
+// Workspace of the many-column path: status word, number of tiles; tiles; order; u.
 #ifndef LORA_CTAS
 #define LORA_CTAS 256
 #endif
@@ -1031,7 +1074,8 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
     p.ntasks = n;
     if (ncols > kClusterCols) {
         uint8_t *ws = static_cast<uint8_t *>(workspace);
-        p.ntiles = reinterpret_cast<int *>(ws);
+        p.status = reinterpret_cast<int *>(ws);
+        p.ntiles = p.status + 1;
         p.tiles = reinterpret_cast<LoraTile *>(ws + L.tiles);
         p.order = reinterpret_cast<int *>(ws + L.order);
         p.u = reinterpret_cast<uint16_t *>(ws + L.u);
@@ -1040,9 +1084,9 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
         // rows per expand CTA: few enough for several CTAs per SM
         int64_t rows = 0;
         for (int i = 0; i < n; ++i) rows += p.task[i].nrows;
-        p.rows_per_cta = 512;
+        p.rows_per_cta = LORA_ROWS;
         const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
-        while (p.rows_per_cta > 64 && tiles * (rows / p.rows_per_cta) < 592) p.rows_per_cta /= 2;
+        while (p.rows_per_cta > kRows && tiles * (rows / p.rows_per_cta) < 592) p.rows_per_cta /= 2;
         while (rows / p.rows_per_cta >= 65535) p.rows_per_cta *= 2;  // (a grid's second dimension)
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
