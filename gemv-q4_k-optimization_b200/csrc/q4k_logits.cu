@@ -33,21 +33,10 @@ struct LogitsParams {
     int slots;  // listed tokens a CTA has room for
 };
 
-#ifndef LG_NC
-#define LG_NC 0
-#endif
-#ifndef LG_T
-#define LG_T 256
-#define LG_Q 4
-#define LG_MB 4
-#endif
-constexpr int kThreads = LG_T;
-constexpr int kQuads = LG_Q;                      // groups of 4 tokens per thread and chunk (at most 8)
+constexpr int kThreads = 256;
+constexpr int kQuads = 4;                         // groups of 4 tokens per thread and chunk (at most 8)
 constexpr int kChunk = kThreads * kQuads * 4;     // tokens in flight per CTA
-#ifndef LG_SEG
-#define LG_SEG 65536
-#endif
-constexpr int kSegment = LG_SEG;                   // tokens whose listed places are held at a time
+constexpr int kSegment = 65536;                   // tokens whose listed places are held at a time
 constexpr int kMinSlots = 256, kMaxSlots = 4096;  // listed tokens with room for their count and bias sum
 constexpr int kAhead = 4;                         // list entries per thread in registers
 constexpr float kLog2e = 1.4426950408889634f;
@@ -235,7 +224,7 @@ __device__ __forceinline__ uint32_t of_row(int v, int v1) {
 // tokens go in one access; quads start on such a boundary (`shift` tokens
 // before a multiple of 4), and only the quads at a row's ends go one by one.
 template <bool V4>
-__global__ void __launch_bounds__(kThreads, LG_MB) k_logits(const __grid_constant__ LogitsParams P) {
+__global__ void __launch_bounds__(kThreads, 4) k_logits(const __grid_constant__ LogitsParams P) {
     extern __shared__ __align__(16) uint8_t smem[];
     Lists &S = *reinterpret_cast<Lists *>(smem);
     __shared__ Stat part[kThreads / 32], all[16];
@@ -440,7 +429,7 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     }
     // eight CTAs for every SM (four are resident: the rest evens out their ends) if the vocabulary has a chunk for each
     int nc = 1;
-    while (nc < 16 && nc * kChunk < p.nvocab && (LG_NC ? nc < LG_NC : nc * static_cast<int64_t>(ncols) < 1184)) nc *= 2;
+    while (nc < 16 && nc * kChunk < p.nvocab && nc * static_cast<int64_t>(ncols) < 1184) nc *= 2;
     // slots for a column's whole history and its likely biases (their number per column is known to the device
     // alone); a CTA whose tokens need more takes them in smaller segments
     const int64_t listed = p.max_history + (p.bias_tokens != nullptr ? 2 * static_cast<int64_t>(p.n_bias) / ncols + 64 : 0);

@@ -64,23 +64,24 @@ __device__ __forceinline__ int rank_of(const LoraTask &t, int a) {
 // 4096 x 4096, 16 bits), and a step's calls are too short for two launches. One
 // launch: the cluster splits K over its CTAs (each reads its slice of every row
 // of A once), the partial u meet over distributed shared memory, and each CTA
-// expands its slice of the rows of B. Columns that share an adapter share the
-// reading: the cluster of every kGroup-th column of an adapter takes the next
-// kGroup of them, the clusters of the others end at once.
+// expands its slice of the rows of B. Where there are more columns than
+// clusters run at once, columns of one adapter share the reading: the cluster
+// of every G-th column of an adapter takes the next G of them, the clusters of
+// the others end at once.
 // What bounds it is the chain of round trips to memory, so it is kept short:
 // ids -> {ranks, scales, x, first A, first B, base} -> partial sums -> cluster
-// barrier -> the other CTAs' parts -> rows.
-#ifndef LORA_T
-#define LORA_T 512
-#define LORA_MB 1
-#endif
-constexpr int kThreads = LORA_T;
+// barrier -> the other CTAs' parts -> rows. In a graph: one column through
+// 4096 x 4096, rank 16, bf16 4.8 us (an empty launch takes about 2); 8 columns
+// of 3 adapters, K = 14336, rank 32, fp32 8.9 us; 64 columns of 16 adapters,
+// 14336 rows 25 us. The same sums on bf16 MMAs (below) measured slower here
+// (one column 5.6, K = 14336 in fp32 11.8 us): cutting weights into pieces
+// costs more than it saves where a weight serves one to four columns.
+// 512 threads on an SM measured faster than two CTAs of 256 where a call has
+// bytes to move (8 columns, K = 14336, fp32: 9.4 against 11.4 us), with 64
+// registers for two CTAs of 512 it spills (9.5 -> 12.3 us).
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kClusterCols = 64;  // columns up to which this kernel runs (bits of a mask)
-#ifndef LORA_G
-#define LORA_G 8
-#endif
-constexpr int kGroup = LORA_G;         // columns of one adapter per cluster
 constexpr int kTile = 1024;       // values of x per column in shared memory at a time
 constexpr int kBatch = 2;         // rows of A per warp and pass
 constexpr int kAhead = 4;         // chunks of a row of B in flight per lane
@@ -108,7 +109,9 @@ template <typename T, int V> __device__ __noinline__ Chunk<T, V> load_end(const 
 template <typename T, int V> __device__ __forceinline__ Chunk<T, V> load_chunk(const T *p, int n) {
     if constexpr (V > 1) {
         if (n < V) return load_end<T, V>(p, n);
-        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p));
+        // (volatile: asked for where it stands, not where it is used)
+        uint4 raw;
+        asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w) : "l"(p));
         return *reinterpret_cast<const Chunk<T, V> *>(&raw);
     } else {
         Chunk<T, V> c;
@@ -236,10 +239,10 @@ __device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, uint
         ask_base();
     }
     cluster.sync();
-    for (int i = tid; i < r * G; i += kThreads) {
+    for (int i = tid; i < (r + VB - 1) / VB * VB * G; i += kThreads) {  // (zeros behind the rank)
         float p[NC], s = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) p[c] = cluster.map_shared_rank(part, c)[i];
+        for (int c = 0; c < NC; ++c) p[c] = i < r * G ? cluster.map_shared_rank(part, c)[i] : 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) s += p[c];
         us[i] = s * scale;
@@ -252,11 +255,15 @@ __device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, uint
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 const int c = c0 + i * L * VB;
+                if (c >= r) break;
+                if (VB > 1 && c + VB > r)  // values behind the rank may be anything (u is zero there)
+#pragma unroll
+                    for (int e = 1; e < VB; ++e)
+                        if (c + e >= r) wb[i].v[e] = T(0.0f);
 #pragma unroll
                 for (int e = 0; e < VB; ++e)
-                    if (c + e < r)
 #pragma unroll
-                        for (int g = 0; g < G; ++g) acc[g] = fmaf(to_f32(wb[i].v[e]), us[(c + e) * G + g], acc[g]);
+                    for (int g = 0; g < G; ++g) acc[g] = fmaf(to_f32(wb[i].v[e]), us[(c + e) * G + g], acc[g]);
             }
             c0 += kAhead * L * VB;
             if (c0 - sub * VB >= r) break;
@@ -277,8 +284,8 @@ __device__ __forceinline__ void lora_group(const LoraTask &t, int a, int r, uint
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <typename T, int VA, int VB, int NC>
-__global__ void __launch_bounds__(kThreads, LORA_MB) k_lora_cluster(const __grid_constant__ LoraParams P) {
+template <typename T, int VA, int VB, int G, int NC>
+__global__ void __launch_bounds__(kThreads) k_lora_cluster(const __grid_constant__ LoraParams P) {
     extern __shared__ __align__(16) float smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const LoraTask &t = P.task[blockIdx.y];
@@ -298,29 +305,23 @@ __global__ void __launch_bounds__(kThreads, LORA_MB) k_lora_cluster(const __grid
     }
     uint64_t mask = __ballot_sync(0xffffffffu, id0 == a) | static_cast<uint64_t>(__ballot_sync(0xffffffffu, id1 == a)) << 32;
     const uint64_t before = mask & ((uint64_t(1) << j) - 1);
-    if (__popcll(before) % kGroup != 0) return;  // another column's cluster does this one (all CTAs agree)
+    if (__popcll(before) % G != 0) return;  // another column's cluster does this one (all CTAs agree)
     mask &= ~before;
-    float *xs = smem, *part = smem + kGroup * kTile, *us = part + kGroup * t.rank;
-    const int count = __popcll(mask);
-    if (count == 1)
-        lora_group<T, VA, VB, 1, NC>(t, a, r, mask, xs, part, us, cluster);
-    else if (count <= 4)
-        lora_group<T, VA, VB, 4, NC>(t, a, r, mask, xs, part, us, cluster);
-    else
-        lora_group<T, VA, VB, kGroup, NC>(t, a, r, mask, xs, part, us, cluster);
+    float *xs = smem, *part = smem + G * kTile, *us = part + G * ((t.rank + 3) & ~3);  // (16-byte aligned)
+    lora_group<T, VA, VB, G, NC>(t, a, r, mask, xs, part, us, cluster);
 }
 
-size_t cluster_smem(int rank) { return (kGroup * kTile + 2 * kGroup * rank) * sizeof(float); }
+size_t cluster_smem(int g, int rank) { return (g * kTile + 2 * static_cast<size_t>(g) * (rank + 8)) * sizeof(float); }
 
-template <typename T, int VA, int VB, int NC>
+template <typename T, int VA, int VB, int G, int NC>
 cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
-    auto *fn = k_lora_cluster<T, VA, VB, NC>;
+    auto *fn = k_lora_cluster<T, VA, VB, G, NC>;
     static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem(Q4K_MAX_LORA_RANK));
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cluster_smem(G, Q4K_MAX_LORA_RANK)));
         if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
@@ -328,7 +329,7 @@ cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStr
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.ncols * NC, ntasks);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = cluster_smem(rank);
+    cfg.dynamicSmemBytes = cluster_smem(G, rank);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -342,12 +343,19 @@ cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStr
 
 template <typename T, int VA, int VB>
 cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
-#ifdef LORA_NC
-    return launch_cluster_of<T, VA, VB, LORA_NC>(p, ntasks, rank, s);
-#else
-    return p.ncols * ntasks <= 18 ? launch_cluster_of<T, VA, VB, 16>(p, ntasks, rank, s)
-                                  : launch_cluster_of<T, VA, VB, 8>(p, ntasks, rank, s);
-#endif
+    // One CTA fits on an SM, so 9 clusters of 16, 18 of 8 or 37 of 4 run at once. As long as a cluster for every column
+    // and task fits, sharing an adapter's bytes (they are in L2) gains less than the columns' arithmetic on one cluster
+    // costs; beyond that the clusters shrink, and then columns share. Measured at rank 32, bf16, K = 4096, us:
+    // 8 columns of one adapter, 1024 rows: one group of 8 11.2, a cluster for each 6.0;
+    // 12 columns of 16 adapters, 4096 rows: clusters of 16 10.9, of 8 6.7;
+    // 24 columns, 14336 rows, clusters of 8 in groups of 2: one adapter 13.0, 16 adapters 22.8; clusters of 4: 16.3 both;
+    // 48 columns of 16 adapters, 4096 rows: clusters of 8 in groups of 4 14.5, of 4 in groups of 2 10.9.
+    const int pieces = p.ncols * ntasks;
+    return pieces <= 9    ? launch_cluster_of<T, VA, VB, 1, 16>(p, ntasks, rank, s)
+           : pieces <= 18 ? launch_cluster_of<T, VA, VB, 1, 8>(p, ntasks, rank, s)
+           : pieces <= 37 ? launch_cluster_of<T, VA, VB, 1, 4>(p, ntasks, rank, s)
+           : pieces <= 48 ? launch_cluster_of<T, VA, VB, 2, 4>(p, ntasks, rank, s)
+                          : launch_cluster_of<T, VA, VB, 4, 4>(p, ntasks, rank, s);
 }
 
 // ---- many columns: grouped products on the tensor cores ----------------------------
@@ -1003,13 +1011,7 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
     return Q4K_OK;
 }
 
-#ifndef LORA_ROWS
-#define LORA_ROWS 512
-#endif
 // Workspace of the many-column path: status word, number of tiles; tiles; order; u.
-#ifndef LORA_CTAS
-#define LORA_CTAS 256
-#endif
 struct LoraLayout {
     size_t tiles = 0, order = 0, u = 0, total = 0;
     int max_slots = 0, u_cols = 0, splits = 1;
@@ -1025,9 +1027,10 @@ LoraLayout lora_layout(const q4k_lora_task *tasks, int ntasks, int ncols) {
         L.u_cols += (tasks[i].rank + 7) / 8 * 8;
         K = std::max(K, tasks[i].K);
     }
-    // K is split until there are about LORA_CTAS CTAs (two or three for each SM), but not below four stages
+    // K is split until there are up to 256 CTAs (two fit on an SM: 4096 columns took 98.7 us at 256, 105.6 at 512, 108.5
+    // at 150), but not below four stages
     const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
-    L.splits = static_cast<int>(std::max<int64_t>(1, std::min({int64_t(kMaxSplits), LORA_CTAS / tiles, K / (4 * kStageK)})));
+    L.splits = static_cast<int>(std::max<int64_t>(1, std::min({int64_t(kMaxSplits), 256 / tiles, K / (4 * kStageK)})));
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     L.tiles = 256;
     L.order = L.tiles + up(static_cast<size_t>(most_tiles(ncols, L.max_slots)) * sizeof(LoraTile));
@@ -1084,7 +1087,7 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
         // rows per expand CTA: few enough for several CTAs per SM
         int64_t rows = 0;
         for (int i = 0; i < n; ++i) rows += p.task[i].nrows;
-        p.rows_per_cta = LORA_ROWS;
+        p.rows_per_cta = 512;
         const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
         while (p.rows_per_cta > kRows && tiles * (rows / p.rows_per_cta) < 592) p.rows_per_cta /= 2;
         while (rows / p.rows_per_cta >= 65535) p.rows_per_cta *= 2;  // (a grid's second dimension)
