@@ -10,6 +10,8 @@ copied to the device once.  GGUF stores a matrix as ne = [K, rows] with rows
 contiguous: exactly the Q4_K row layout, so no repacking is needed.
 
 Names follow llama.cpp's tensor naming (`blk.{i}.attn_q.weight`, ...).
+Adapter files (`load_adapters`) and the rotary parameters (`GGUFModel.rope`)
+come the same way, in the form q4k.lora_batch and q4k.rope_multi take.
 """
 from __future__ import annotations
 
@@ -69,6 +71,38 @@ class GGUFModel:
             return int(n)
         idx = {int(name.split(".")[1]) for name in self.tensors if name.startswith("blk.")}
         return max(idx) + 1 if idx else 0
+
+    def array(self, key: str) -> list | None:
+        """An array metadata value as a list (None when absent)."""
+        f = self.reader.fields.get(key)
+        if f is None:
+            return None
+        return [v for i in f.data for v in np.asarray(f.parts[i]).tolist()]
+
+    def rope(self, q4k, layout: str | None = None, order: str = "blocks", device="cuda") -> dict:
+        """Keyword arguments for q4k.rope_multi (inv_freq, sections, layout, order) from the
+        metadata `<arch>.rope.*` and the `rope_freqs.weight` factors.  Sections are the
+        M-RoPE `dimension_sections` without trailing zeros (one axis where there are none).
+        layout: "adjacent" for llama files (their q and k rows are stored for neighbouring
+        pairs), else "half", unless given."""
+        a = self.arch
+        n_rot = self.field(f"{a}.rope.dimension_count")
+        if n_rot is None:
+            heads, width = self.field(f"{a}.attention.head_count"), self.field(f"{a}.embedding_length")
+            if not heads or not width:
+                raise KeyError(f"{self.path}: no {a}.rope.dimension_count")
+            n_rot = int(width) // int(heads)
+        base = self.field(f"{a}.rope.freq_base") or 10000.0
+        factor = self.field(f"{a}.rope.scaling.factor")
+        linear = self.field(f"{a}.rope.scaling.type") == "linear"
+        scale = 1.0 / factor if linear and factor else 1.0
+        t = self.tensors.get("rope_freqs.weight")
+        sections = [int(v) for v in self.array(f"{a}.rope.dimension_sections") or []]
+        while sections and sections[-1] == 0:
+            sections.pop()
+        return dict(inv_freq=q4k.rope_inv_freq(int(n_rot), base, scale, None if t is None else np.array(t.data), device=device),
+                    sections=tuple(sections) or (int(n_rot) // 2,),
+                    layout=layout or ("adjacent" if a == "llama" else "half"), order=order)
 
     # ---- tensors ----------------------------------------------------------
     def q4k(self, name: str) -> Q4KTensor:
@@ -132,13 +166,107 @@ def layer_tasks(q4k, layer: dict[str, Q4KTensor], xs: dict, outs: dict, fuse_ffn
     return q4k.make_tasks_ex(items)
 
 
+# ---- low-rank adapters -----------------------------------------------------------
+def load_adapters(paths, names, device="cuda", dtype=None, strengths=None) -> dict[str, dict]:
+    """Adapter files (llama.cpp's `adapter.type = lora`: `<tensor>.lora_a` with ne = [K, rank],
+    `<tensor>.lora_b` with ne = [rank, rows]) stacked into slots, slot s = paths[s], for the
+    matrices `names` (e.g. "blk.0.attn_q.weight"): name -> dict(A, B, ranks, scales) as
+    q4k.lora_batch takes them, in `dtype` (default: fp16).  The scale of a slot is
+    strengths[s] * alpha / rank (strengths[s] where the file's alpha is 0 or missing); a
+    matrix that a file does not adapt has rank 0 in its slot; ranks are padded to a
+    multiple of 8 so that rows stay 16-byte aligned.  Matrices that no file adapts are
+    left out."""
+    import gguf
+    import torch
+    dtype = torch.float16 if dtype is None else dtype
+    files = []
+    for path in paths:
+        m = GGUFModel(path)
+        if m.field("adapter.type") not in (None, "lora"):
+            raise TypeError(f"{path}: adapter.type {m.field('adapter.type')!r}, not lora")
+        files.append((m, float(m.field("adapter.lora.alpha") or 0.0)))
+    strengths = [1.0] * len(files) if strengths is None else list(strengths)
+    if len(strengths) != len(files):
+        raise ValueError(f"{len(strengths)} strengths for {len(files)} adapters")
+
+    def matrix(t) -> np.ndarray:
+        if t.tensor_type in (gguf.GGMLQuantizationType.F32, gguf.GGMLQuantizationType.F16):
+            a = np.asarray(t.data).astype(np.float32)
+        else:  # bf16 and quantized adapters
+            a = gguf.quants.dequantize(np.asarray(t.data), t.tensor_type)
+        return np.ascontiguousarray(a.reshape([int(d) for d in t.shape][::-1][-2:]))
+
+    out = {}
+    for name in names:
+        pairs = []
+        for m, _ in files:
+            a, b = m.tensors.get(name + ".lora_a"), m.tensors.get(name + ".lora_b")
+            if (a is None) != (b is None):
+                raise KeyError(f"{m.path}: {name} has only one of lora_a and lora_b")
+            pairs.append(None if a is None else (matrix(a), matrix(b)))
+        some = [p for p in pairs if p is not None]
+        if not some:
+            continue
+        K, rows = some[0][0].shape[1], some[0][1].shape[0]
+        for (m, _), p in zip(files, pairs):
+            if p is not None and (p[0].shape[1] != K or p[1].shape != (rows, p[0].shape[0])):
+                raise ValueError(f"{m.path}: {name}: shapes {p[0].shape} and {p[1].shape}")
+        rank = (max(p[0].shape[0] for p in some) + 7) // 8 * 8
+        A, B = torch.zeros((len(files), rank, K), dtype=dtype), torch.zeros((len(files), rows, rank), dtype=dtype)
+        ranks, scales = torch.zeros(len(files), dtype=torch.int32), torch.zeros(len(files), dtype=torch.float32)
+        for s, p in enumerate(pairs):
+            if p is None:
+                continue
+            r = p[0].shape[0]
+            A[s, :r], B[s, :, :r] = torch.from_numpy(p[0]).to(dtype), torch.from_numpy(p[1]).to(dtype)
+            ranks[s] = r
+            scales[s] = strengths[s] * (files[s][1] / r if files[s][1] and r else 1.0)
+        out[name] = dict(A=A.to(device), B=B.to(device), ranks=ranks.to(device), scales=scales.to(device))
+    return out
+
+
+def layer_adapter_items(adapters: dict[str, dict], i: int, xs: dict, outs: dict) -> list[dict]:
+    """Items for q4k.lora_batch that add the adapters of decoder layer i to the outputs of its
+    layer_tasks launch, in place (xs, outs: as for layer_tasks, unfused)."""
+    items = []
+    for key, stem, grp in LLAMA_LAYER:
+        ad = adapters.get(f"blk.{i}.{stem}.weight")
+        if ad is not None and key in outs:
+            items.append(dict(x=xs[grp], base=outs[key], out=outs[key], **ad))
+    return items
+
+
+def write_adapter_gguf(path: str | Path, mats: dict[str, tuple[np.ndarray, np.ndarray]], alpha: float,
+                       arch: str = "llama") -> None:
+    """Write an adapter file: name -> (A (rank, K), B (rows, rank)) in fp16 or fp32."""
+    import gguf
+    w = gguf.GGUFWriter(str(path), arch)
+    w.add_string("general.type", "adapter")
+    w.add_string("adapter.type", "lora")
+    w.add_float32("adapter.lora.alpha", float(alpha))
+    for name, (a, b) in mats.items():
+        w.add_tensor(name + ".lora_a", np.ascontiguousarray(a))
+        w.add_tensor(name + ".lora_b", np.ascontiguousarray(b))
+    w.write_header_to_file()
+    w.write_kv_data_to_file()
+    w.write_tensors_to_file()
+    w.close()
+
+
 def write_q4k_gguf(path: str | Path, tensors: dict[str, np.ndarray], arch: str = "llama",
-                   extra_f32: dict[str, np.ndarray] | None = None, n_layers: int | None = None) -> None:
+                   extra_f32: dict[str, np.ndarray] | None = None, n_layers: int | None = None,
+                   metadata: dict | None = None) -> None:
     """Write a GGUF file holding Q4_K matrices given as (rows, K/256*144) uint8
-    arrays (and optional fp32 tensors): for tests and for staging synthetic
+    arrays (and optional fp32 tensors, and metadata of whole numbers, fp32,
+    strings and lists of whole numbers): for tests and for staging synthetic
     weights in the on-disk format."""
     import gguf
     w = gguf.GGUFWriter(str(path), arch)
+    for key, v in (metadata or {}).items():
+        if isinstance(v, (list, tuple)):
+            w.add_array(key, list(v))
+        else:
+            {int: w.add_uint32, float: w.add_float32, str: w.add_string}[type(v)](key, v)
     if n_layers is not None:
         w.add_block_count(n_layers)
     for name, a in tensors.items():
