@@ -11,6 +11,13 @@ function names follow the reference entry points they stand in for
   quantize_row_q8_1    quantize_row_q8_1_cuda call   kernels/mmvq.cu:734
   custom_q4k_gemv      custom_q4k_gemv hook launch   kernels/mmvq.cu:10-18, :563-584
 
+What each request of a batch brings of its own (no counterpart in the
+reference) goes through the native front-end _q4k_torch.so:
+
+  lora_add, lora_batch         low-rank adapters beside the shared projections
+  rope_multi                   rotary positions with several axes
+  logits_process               penalties, biases and masks on the logits
+
 Tensor conventions: a Q4_K matrix is a uint8 tensor (nrows, K/256*144);
 fp32 activations are (ncols, K) (column j = row j of the tensor, so the ggml
 column stride is x.stride(0)); outputs are (ncols, nrows).  There is no CPU

@@ -1,6 +1,7 @@
 // q4k_logits.cu -- q4k_logits_process: penalties for repeated tokens, biases
 // and masks on the head's logits, the greedy token and the log-sum-exp of the
 // result, in one pass.
+#include "q4k_device.cuh"
 #include "q4k_request.h"
 
 #include <cooperative_groups.h>
@@ -233,6 +234,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_logits(const __grid_constant__ 
     const int64_t j = blockIdx.x / nc;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // (waited for below: every CTA has begun)
+    pdl_launch_dependents();
+    pdl_wait();
     const float *l = P.logits + j * P.s_col;
     float *d = P.dst + j * P.s_dst;
     // this CTA's tokens [v0, v1): whole quads of the row's alignment
@@ -435,19 +438,8 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     const int64_t listed = p.max_history + (p.bias_tokens != nullptr ? 2 * static_cast<int64_t>(p.n_bias) / ncols + 64 : 0);
     LogitsParams q = p;
     q.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, std::max<int64_t>(kMinSlots, (listed + 31) / 32 * 32)));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(ncols) * nc);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.history != nullptr || p.bias_tokens != nullptr ? list_bytes(q.slots) : 0;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = nc;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, q);
+    const size_t smem = p.history != nullptr || p.bias_tokens != nullptr ? list_bytes(q.slots) : 0;
+    return launch_request(fn, dim3(static_cast<unsigned>(ncols) * nc), kThreads, smem, dim3(nc), q, s);
 }
 
 }  // namespace

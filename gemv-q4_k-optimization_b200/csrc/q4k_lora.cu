@@ -288,6 +288,8 @@ template <typename T, int VA, int VB, int G, int NC>
 __global__ void __launch_bounds__(kThreads) k_lora_cluster(const __grid_constant__ LoraParams P) {
     extern __shared__ __align__(16) float smem[];
     cg::cluster_group cluster = cg::this_cluster();
+    pdl_launch_dependents();
+    pdl_wait();
     const LoraTask &t = P.task[blockIdx.y];
     const int j = blockIdx.x / NC;
     const int tid = threadIdx.x, lane = tid & 31;
@@ -326,19 +328,7 @@ cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStr
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.ncols * NC, ntasks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = cluster_smem(G, rank);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = NC;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, p);
+    return launch_request(fn, dim3(p.ncols * NC, ntasks), kThreads, cluster_smem(G, rank), dim3(NC), p, s);
 }
 
 template <typename T, int VA, int VB>
@@ -466,6 +456,7 @@ __device__ __forceinline__ void products(float (&acc)[4][4], const uint32_t (&a)
 __global__ void __launch_bounds__(1024) k_lora_plan(const __grid_constant__ LoraParams P) {
     __shared__ int bin[Q4K_MAX_LORA_SLOTS + 1], at[Q4K_MAX_LORA_SLOTS + 1], warps[2][32];
     pdl_launch_dependents();
+    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, bins = P.max_slots + 1;
     auto bin_of = [&](int j) {
         const int id = P.ids[j];
@@ -855,26 +846,6 @@ __global__ void __launch_bounds__(256, 3) k_lora_expand(const __grid_constant__ 
 }
 
 template <typename T> constexpr size_t kShrinkSmem = kRing * kShrinkStage<T>;
-// A launch that may begin while the one before it ends (its kernel waits for it).
-template <typename K>
-cudaError_t launch_next(K *fn, dim3 grid, int cluster_y, int threads, size_t smem, const LoraParams &p, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1;
-    attr[1].val.clusterDim.y = cluster_y;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster_y > 0 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, fn, p);
-}
-
 // Tiles there can be: whole ones, and one begun per bin.
 int most_tiles(int ncols, int max_slots) { return ncols / kTileCols + (ncols < max_slots + 1 ? ncols : max_slots + 1); }
 
@@ -897,19 +868,18 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, cudaS
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
     const unsigned tiles = static_cast<unsigned>(most_tiles(p.ncols, p.max_slots));
-    k_lora_plan<<<1, 1024, 0, s>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if ((e = launch_request(k_lora_plan, dim3(1), 1024, 0, dim3(0), p, s)) != cudaSuccess) return e;
     unsigned chunks = 0, rows = 0;
     for (int i = 0; i < p.ntasks; ++i) {
         chunks += (p.task[i].rank + kRanks - 1) / kRanks;
         rows = std::max(rows, static_cast<unsigned>(p.task[i].nrows));
     }
     if (chunks > 0) {
-        e = launch_next(shrink, dim3(tiles, p.splits, chunks), p.splits, 256, kShrinkSmem<T>, p, s);
+        e = launch_request(shrink, dim3(tiles, p.splits, chunks), 256, kShrinkSmem<T>, dim3(1, p.splits), p, s);
         if (e != cudaSuccess) return e;
     }
-    return launch_next(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 0, 256,
-                       kExpandSmem<T>, p, s);
+    return launch_request(expand, dim3(tiles, (rows + p.rows_per_cta - 1) / p.rows_per_cta, p.ntasks), 256, kExpandSmem<T>,
+                          dim3(0), p, s);
 }
 
 // Whether every run of 8 values of every row is 16-byte aligned.

@@ -57,4 +57,26 @@ inline bool runs_overlap(const Runs &a, const Runs &b) {
     return d < a.len || a.stride - d < b.len;
 }
 
+// A launch that may begin while the one before it on the stream ends: its kernel
+// waits for that one (griddepcontrol.wait) before it touches memory. cluster:
+// 0 in x for none.
+template <typename P>
+cudaError_t launch_request(void (*fn)(P), dim3 grid, int threads, size_t smem, dim3 cluster, const P &p, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster.x > 0 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
 }  // namespace q4k

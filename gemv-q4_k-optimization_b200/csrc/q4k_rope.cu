@@ -6,6 +6,7 @@
 // The angle is formed in fp64 as a number of half turns and reduced there
 // (a far position times an inverse frequency holds more digits than fp32
 // keeps); its sine and cosine are fp32.
+#include "q4k_device.cuh"
 #include "q4k_request.h"
 
 #include <cuda_bf16.h>
@@ -65,6 +66,8 @@ constexpr int kThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_rope(const __grid_constant__ RopeParams P) {
     __shared__ float2 cs[Q4K_MAX_ROPE_DIM / 2];
+    pdl_launch_dependents();
+    pdl_wait();
     const int64_t j = blockIdx.x;
     const int half = P.n_rot / 2;
     for (int i = threadIdx.x; i < half; i += kThreads) cs[i] = turn_of(P, i, j);
@@ -111,6 +114,8 @@ template <typename T> __device__ __forceinline__ void store4(T *d, const float (
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(kThreads) k_rope_vec(const __grid_constant__ RopeParams P) {
     __shared__ float2 cs[Q4K_MAX_ROPE_DIM / 2];
+    pdl_launch_dependents();
+    pdl_wait();
     const int64_t j = blockIdx.x;
     const int half = P.n_rot / 2, groups = half / 4 + (P.head_dim - P.n_rot) / 8;
     const int g = threadIdx.x & (P.lanes - 1), step = kThreads / P.lanes;  // lanes: groups, up to a power of two
@@ -177,10 +182,7 @@ template <typename T> cudaError_t launch_rope(RopeParams &p, int ncols, cudaStre
         vec = vec && aligned_to(t.x, 16) && t.sx_col % 4 == 0 && t.sx_head % 4 == 0 && aligned_to(t.dst, 4 * sizeof(T)) &&
               t.sd_col % 4 == 0 && t.sd_head % 4 == 0;
     }
-    if (!vec) {
-        k_rope<T><<<ncols, kThreads, 0, s>>>(p);
-        return cudaGetLastError();
-    }
+    if (!vec) return launch_request(k_rope<T>, dim3(ncols), kThreads, 0, dim3(0), p, s);
     p.lanes = 1;
     while (p.lanes < groups) p.lanes *= 2;
     const int step = kThreads / p.lanes;
@@ -189,11 +191,7 @@ template <typename T> cudaError_t launch_rope(RopeParams &p, int ncols, cudaStre
     p.heads_per_block = ncols >= 592 ? p.heads : step;
     while (p.heads / p.heads_per_block >= 65535) p.heads_per_block *= 2;  // (a grid's second dimension)
     const dim3 grid(ncols, (p.heads + p.heads_per_block - 1) / p.heads_per_block);
-    if (p.layout == Q4K_ROPE_HALF)
-        k_rope_vec<T, true><<<grid, kThreads, 0, s>>>(p);
-    else
-        k_rope_vec<T, false><<<grid, kThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_request(p.layout == Q4K_ROPE_HALF ? k_rope_vec<T, true> : k_rope_vec<T, false>, grid, kThreads, 0, dim3(0), p, s);
 }
 
 // heads x ncols runs of dim values: apart when one of the two strides steps over the other's whole span.

@@ -376,7 +376,9 @@ Q4K_API size_t q4k_noalloc_scratch_bytes(void);
 /* A batch's columns share the weights above; three things belong to the
  * request behind each column: its low-rank adapter, its rotary positions and
  * the controls on its logits.  The entries below take these as device arrays
- * indexed by column, so one captured graph serves changing requests.  No
+ * indexed by column, so one captured graph serves changing requests.  All
+ * launches are programmatic dependents of the stream's previous one and wait
+ * for it before they touch memory.  No
  * counterpart in the reference (upstream llama.cpp runs them as separate graph
  * nodes or on the host).  They take any number of columns (ncols 0: nothing
  * to do), keep nothing between calls and give the same bits every time. */
@@ -418,7 +420,10 @@ typedef struct q4k_lora_task {
 #define Q4K_MAX_LORA_SLOTS 1024
 #define Q4K_MAX_LORA_RANK 512
 /* Every task's adapters for all columns; ids (ncols device ints) serves all
- * tasks (at most Q4K_MAX_TASKS).  The workspace need not be initialised. */
+ * tasks (at most Q4K_MAX_TASKS).  Up to 64 columns take one launch and no
+ * workspace (q4k_lora_workspace_bytes 0); more take three launches, whose
+ * workspace need not be initialised (a wait that gives up after 2 s leaves
+ * Q4K_ETIMEOUT in its status word, see q4k_workspace_status). */
 Q4K_API size_t q4k_lora_workspace_bytes(const q4k_lora_task *tasks, int ntasks, int ncols);
 Q4K_API int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int32_t *ids, void *workspace,
                            size_t workspace_bytes, q4k_stream_t stream);
@@ -461,7 +466,7 @@ Q4K_API int q4k_rope_multi(const q4k_rope_tensor *tensors, int ntensors, int nco
  * column j and token v, in fp32:
  *   z = logits[j][v] + sum of the biases of column j at v, added up first, in list order;
  *   if v occurs c > 0 times in the history of column j:
- *       z = z > 0 ? z / repeat : z * repeat;  z = z - (c * frequency + presence);
+ *       z = z > 0 ? z / repeat : z * repeat;  z = z - (c * frequency + presence);  (repeat > 0)
  *   if column j's mask has bit v clear: z = -inf, whatever z was.
  * token[j]: the lowest index with the largest z above -inf (NaN is never
  * picked), or -1; lse[j] = log(sum_v exp(z)): -inf when nothing is left. */

@@ -75,6 +75,7 @@ SHAPES = [  # ncols, K, N, slots, rank: one token and one value up to batches, w
     (8, 4096, 1024, 8, 64), (8, 14336, 512, 3, 33), (9, 512, 300, 4, 128), (13, 100, 4097, 2, 200), (17, 2048, 512, 20, 16),
     (33, 320, 72, 3, 64), (64, 1024, 2048, 7, 32), (65, 513, 257, 5, 24), (100, 96, 1100, 9, 512), (130, 2048, 640, 2, 72),
     (300, 1000, 513, 40, 24), (777, 128, 130, 6, 9), (1024, 512, 256, 3, 64), (2500, 72, 65, 1000, 4),
+    (64, 48, 200, 1024, 16), (600, 40, 33, 1024, 8),
 ]
 
 
@@ -284,6 +285,21 @@ def test_lora_beside_the_projection_it_adapts(q4k, oracle):
     # the GEMV's bar, and the adapter's fp32 sums: n additions of terms up to the sum of magnitudes
     mag = reference({**d, "x": d["x"].abs(), "A": d["A"].abs(), "B": d["B"].abs(), "base": d["base"].abs()})
     assert ((y.double() - want).abs() <= 1e-4 + 1e-5 * want.abs() + 1041 ** 0.5 * 2.0 ** -24 * mag).all()
+
+
+def test_lora_workspace_of_the_caller_reports_ok(q4k):
+    """Many columns in a caller's workspace with any contents: the call leaves its status word at 0."""
+    import torch
+    d = make(9, 200, 256, 96, 3, 8, "float16")
+    ws = q4k.Workspace(1 << 20)
+    ws.buf.fill_(255)
+    got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], base=d["base"], ranks=d["ranks"], scales=d["scales"], ws=ws)
+    check_exact(got, reference(d))
+    assert ws.status() == 0
+    big = make(10, 3000, 256, 96, 3, 8, "float16")  # grows on demand
+    got = q4k.lora_add(big["x"], big["A"], big["B"], big["ids"], base=big["base"], ranks=big["ranks"], scales=big["scales"], ws=ws)
+    check_exact(got, reference(big))
+    assert ws.status() == 0
 
 
 def test_lora_empty_calls(q4k):
