@@ -114,11 +114,6 @@ __device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C
     int *count = S.token + slots, *biases = count + slots;
     float *bias = reinterpret_cast<float *>(biases + slots);
     for (int i = tid; i < words; i += kThreads) S.touched[i] = 0u;
-    for (int i = tid; i < slots; i += kThreads) {
-        count[i] = 0;
-        biases[i] = 0;
-        bias[i] = 0.0f;
-    }
     if (tid == 0) S.repeats = 0;
     __syncthreads();
     auto in = [&](int tok) { return tok >= 0 && tok >= base && tok - base < n; };
@@ -145,12 +140,17 @@ __device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C
         if (w < tid / 32) at += S.sums[w];
         total += S.sums[w];
     }
+    if (static_cast<int>(total) > slots) return static_cast<int>(total);
     for (int w = w0; w < w1; ++w) {
         S.before[w] = static_cast<uint16_t>(at);
         at += __popc(S.touched[w]);
     }
+    for (int i = tid; i < static_cast<int>(total); i += kThreads) {
+        count[i] = 0;
+        biases[i] = 0;
+        bias[i] = 0.0f;
+    }
     __syncthreads();
-    if (static_cast<int>(total) > slots) return static_cast<int>(total);
     auto slot = [&](int tok) {
         const int i = tok - base;
         return S.before[i >> 5] + __popc(S.touched[i >> 5] & ((1u << (i & 31)) - 1u));

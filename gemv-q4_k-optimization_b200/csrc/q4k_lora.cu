@@ -704,8 +704,10 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
     return true;
 }
 
+// Four CTAs per SM overlap one another's chain (operands -> MMAs -> base -> dst):
+// 4096 columns took 73.1 us with three, 70.2 with four, 75.7 with five (whole call).
 template <typename T, bool VB>
-__global__ void __launch_bounds__(256, 3) k_lora_expand(const __grid_constant__ LoraParams P) {
+__global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ LoraParams P) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ struct {
         const float *base;

@@ -287,6 +287,35 @@ def test_lora_beside_the_projection_it_adapts(q4k, oracle):
     assert ((y.double() - want).abs() <= 1e-4 + 1e-5 * want.abs() + 1041 ** 0.5 * 2.0 ** -24 * mag).all()
 
 
+@pytest.mark.parametrize("ncols", [24, 64, 700])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lora_gives_the_same_bits_every_time(q4k, ncols, dtype):
+    """Repeated calls agree bit for bit, and a column's result does not depend on the columns beside it
+    within the same launch path."""
+    import torch
+    d = make(ncols, ncols, 1000, 384, 5, 40, dtype, exact=False)
+    run = lambda x, ids: q4k.lora_add(x, d["A"], d["B"], ids, ranks=d["ranks"], scales=d["scales"])  # noqa: E731
+    first = run(d["x"], d["ids"])
+    for _ in range(5):
+        assert torch.equal(run(d["x"], d["ids"]), first)
+    perm = torch.randperm(ncols, device="cuda")
+    assert torch.equal(run(d["x"][perm], d["ids"][perm]), first[perm])
+
+
+@pytest.mark.parametrize("ncols", [3, 100])
+def test_lora_nothing_to_add(q4k, ncols):
+    """No ranks, no slots, no K, ranks of 0 in use: dst is base, x and the adapters are not read."""
+    import torch
+    d = make(2, ncols, 64, 45, 3, 8, "float16")
+    nan = torch.full_like(d["x"], float("nan"))
+    for kw in (dict(A=d["A"][:, :0], B=d["B"][:, :, :0]), dict(A=d["A"][:0], B=d["B"][:0]),
+               dict(x=d["x"][:, :0], A=d["A"][:, :, :0], B=d["B"]),
+               dict(x=nan, A=d["A"], B=d["B"], ranks=torch.zeros(3, dtype=torch.int32, device="cuda"))):
+        x = kw.pop("x", d["x"])
+        assert torch.equal(q4k.lora_add(x, ids=d["ids"], base=d["base"], **kw), d["base"])
+        assert (q4k.lora_add(x, ids=d["ids"], **kw) == 0).all()
+
+
 def test_lora_workspace_of_the_caller_reports_ok(q4k):
     """Many columns in a caller's workspace with any contents: the call leaves its status word at 0."""
     import torch
