@@ -69,10 +69,12 @@ __device__ __forceinline__ int rank_of(const LoraTask &t, int a) {
 // of every G-th column of an adapter takes the next G of them, the clusters of
 // the others end at once.
 // What bounds it is the chain of round trips to memory, so it is kept short:
-// ids -> {ranks, scales, x, first A, first B, base} -> partial sums -> cluster
-// barrier -> the other CTAs' parts -> rows. In a graph: one column through
+// ids -> rank -> {scale, x, first A, first B, base} -> partial sums -> cluster
+// barrier -> the other CTAs' parts -> rows. (Asking for A and B before the rank
+// is known, as far as the slots have room, gained nothing and cost 1 us at K =
+// 14336.) In a graph: one column through
 // 4096 x 4096, rank 16, bf16 4.8 us (an empty launch takes about 2); 8 columns
-// of 3 adapters, K = 14336, rank 32, fp32 8.9 us; 64 columns of 16 adapters,
+// of 3 adapters, K = 14336, rank 32, fp32 8.7 us; 64 columns of 16 adapters,
 // 14336 rows 25 us. The same sums on bf16 MMAs (below) measured slower here
 // (one column 5.6, K = 14336 in fp32 11.8 us): cutting weights into pieces
 // costs more than it saves where a weight serves one to four columns.
@@ -518,13 +520,19 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, int bytes
                  : "memory");
 }
 
+__device__ __forceinline__ void cp_async4(void *dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src),
+                 "r"(bytes)
+                 : "memory");
+}
+
 // Stage of the shrink's ring: kStageK values of kTileCols columns of x, and of
 // kRanks rows of A as kStageK / 32 slabs of 32. Pitches let the eight rows and
 // four eights of a fragment load meet different banks.
 constexpr int kXPitch = kStageK + 4;
 constexpr int kStageValues = kRanks * kStageK;
 template <typename T> constexpr size_t kShrinkStage = kTileCols * kXPitch * 4 + kStageValues * sizeof(T);
-constexpr int kMaxSplits = 8;  // CTAs that share a tile's K: a cluster
+constexpr int kMaxSplits = 16;  // CTAs that share a tile's K: a cluster
 
 // u of a tile's columns for kRanks ranks. The cluster splits K; in a CTA four
 // pairs of warps take 16 columns each, a warp one half of every stage. x and A come through a ring; lane q of a row
@@ -564,10 +572,10 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
                 for (int row = tid / 16; row < tile.count; row += 16)
                     cp_async16(xs + row * kXPitch + k, left > 0 ? xcol[row] + k0 + k : xcol[row], left > 0 ? left * 4 : 0);
             } else {
-                for (int i = tid; i < tile.count * kStageK; i += 256) {
-                    const int row = i / kStageK, k = i % kStageK;
-                    xs[row * kXPitch + k] = k0 + k < t.K ? xcol[row][k0 + k] : 0.0f;
-                }
+                const int k = tid % kStageK;
+                const bool some = k0 + k < t.K;
+                for (int row = tid / kStageK; row < tile.count; row += 256 / kStageK)
+                    cp_async4(xs + row * kXPitch + k, some ? xcol[row] + k0 + k : xcol[row], some ? 4 : 0);
             }
             if constexpr (VA) {
                 constexpr int E = 16 / sizeof(T), C = kStageK / E;  // values per copy, copies per row
@@ -578,10 +586,16 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
                                some ? left * static_cast<int>(sizeof(T)) : 0);
                 }
             } else {
-                for (int i = tid; i < kRanks * kStageK; i += 256) {
-                    const int row = i / kStageK, k = i % kStageK;
-                    as[((k / 32) * kRanks + row) * 32 + k % 32] = row < nr && k0 + k < t.K ? A[row * t.sa_row + k0 + k] : T(0.0f);
+                const int k = tid % kStageK;
+                T v[kRanks * kStageK / 256];  // (all asked for before the first is stored)
+#pragma unroll
+                for (int i = 0; i < kRanks * kStageK / 256; ++i) {
+                    const int row = tid / kStageK + i * (256 / kStageK);
+                    v[i] = row < nr && k0 + k < t.K ? A[row * t.sa_row + k0 + k] : T(0.0f);
                 }
+#pragma unroll
+                for (int i = 0; i < kRanks * kStageK / 256; ++i)
+                    as[((k / 32) * kRanks + tid / kStageK + i * (256 / kStageK)) * 32 + k % 32] = v[i];
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -863,8 +877,10 @@ cudaError_t launch_grouped(const LoraParams &p, bool vx, bool va, bool vb, cudaS
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
         const int ss = static_cast<int>(kShrinkSmem<T>), es = static_cast<int>(kExpandSmem<T>);
         for (auto *f : {k_lora_shrink<T, true, true>, k_lora_shrink<T, true, false>, k_lora_shrink<T, false, true>,
-                        k_lora_shrink<T, false, false>})
+                        k_lora_shrink<T, false, false>}) {
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ss)) != cudaSuccess) return e;
+            if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        }
         for (auto *f : {k_lora_expand<T, true>, k_lora_expand<T, false>})
             if ((e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, es)) != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
