@@ -117,7 +117,8 @@ __device__ __forceinline__ int scan_lists(const LogitsParams &P, const Column &C
     for (int i = tid; i < words; i += kThreads) S.touched[i] = 0u;
     if (tid == 0) S.repeats = 0;
     __syncthreads();
-    auto in = [&](int tok) { return tok >= 0 && tok >= base && tok - base < n; };
+    // (base + n is at most the vocabulary; base can be below 0, where tok - base would overflow for the largest tok)
+    auto in = [&](int tok) { return tok >= 0 && tok >= base && tok < base + n; };
     auto mark = [&](int tok) {
         if (in(tok)) atomicOr(&S.touched[(tok - base) >> 5], 1u << ((tok - base) & 31));
     };

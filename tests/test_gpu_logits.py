@@ -289,3 +289,23 @@ def test_logits_refusals_of_the_wrapper(q4k):
                dict(mask=None), dict(out=t["logits"][:, :50]), dict(history=t["history"].cpu())):
         with pytest.raises(q4k.Q4KError):
             q4k.logits_process(**{**t, **kw})
+
+
+@pytest.mark.parametrize("off", [0, 1, 2, 3])
+@pytest.mark.parametrize("V", [20, 70001])
+def test_logits_largest_ids_in_lists_are_ignored(q4k, V, off):
+    """Ids up to the largest int32 (padding of some tokenizers) in histories and biases, on rows that begin at every
+    offset from a 16-byte boundary: the tokens before such a row's first one have places below 0."""
+    import torch
+    d = make(V + off, 4, V, hist=40, bias=30)
+    for k in ("history", "bias_tokens"):
+        flat = d[k].reshape(-1)
+        flat[::4] = 2**31 - 1
+        flat[1::8] = 2**31 - 4
+        flat[5::8] = -2**31
+    t = device(d)
+    buf = torch.empty((4, V + 8 - (V + 8) % 4), device="cuda")
+    logits = buf[:, off:off + V]
+    logits.copy_(t.pop("logits"))
+    out = torch.empty_like(buf)[:, off:off + V]
+    check(q4k.logits_process(logits, **t, out=out, pick=True), d)
