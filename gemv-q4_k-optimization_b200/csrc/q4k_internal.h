@@ -18,6 +18,11 @@ constexpr int kMaxTasks = 16;
 constexpr int kMaxGated = 4;  // tasks with a fused gate per launch (their tensor maps are kernel parameters)
 constexpr int kMaxJobs = 16;
 constexpr int kMaxPeers = 8;
+// Start of every workspace: the header (status and sync words, 256 bytes), then
+// split counters of up to 16384 row groups, which the single-launch GEMV leaves
+// zero for its next call. Nothing else may be put there.
+constexpr int kHeaderBytes = 256;
+constexpr int kControlBytes = kHeaderBytes + 16384 * 4;
 
 // GEMV geometry.  A "worker" is one warp; it owns a contiguous range of
 // "atoms" (32 weight rows x kKS super-blocks, plus the kKS activation records

@@ -4,6 +4,7 @@
 //   u[j][t]   = scale_a * sum_k A_a[t][k] x[j][k]        (shrink)
 //   dst[j][n] = base[j][n] + sum_t B_a[n][t] u[j][t]     (expand), a = ids[j]
 #include "q4k_device.cuh"
+#include "q4k_internal.h"
 #include "q4k_request.h"
 
 #include <cooperative_groups.h>
@@ -999,9 +1000,10 @@ int check_tasks(const q4k_lora_task *tasks, int ntasks, int ncols) {
     return Q4K_OK;
 }
 
-// Workspace of the many-column path: status word, number of tiles; tiles; order; u.
+// Workspace of the many-column path: status word; behind the control words, which stay as they are (another call
+// on the same workspace may rely on them): number of tiles; tiles; order; u.
 struct LoraLayout {
-    size_t tiles = 0, order = 0, u = 0, total = 0;
+    size_t ntiles = 0, tiles = 0, order = 0, u = 0, total = 0;
     int max_slots = 0, u_cols = 0, splits = 1;
 };
 
@@ -1020,7 +1022,8 @@ LoraLayout lora_layout(const q4k_lora_task *tasks, int ntasks, int ncols) {
     const int64_t tiles = (ncols + kTileCols - 1) / kTileCols;
     L.splits = static_cast<int>(std::max<int64_t>(1, std::min({int64_t(kMaxSplits), 256 / tiles, K / (4 * kStageK)})));
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    L.tiles = 256;
+    L.ntiles = kControlBytes;
+    L.tiles = L.ntiles + 256;
     L.order = L.tiles + up(static_cast<size_t>(most_tiles(ncols, L.max_slots)) * sizeof(LoraTile));
     L.u = L.order + up(static_cast<size_t>(ncols) * 4);
     L.total = L.u + up(static_cast<size_t>(3) * ncols * L.u_cols * 2);
@@ -1066,7 +1069,7 @@ int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int3
     if (ncols > kClusterCols) {
         uint8_t *ws = static_cast<uint8_t *>(workspace);
         p.status = reinterpret_cast<int *>(ws);
-        p.ntiles = p.status + 1;
+        p.ntiles = reinterpret_cast<int *>(ws + L.ntiles);
         p.tiles = reinterpret_cast<LoraTile *>(ws + L.tiles);
         p.order = reinterpret_cast<int *>(ws + L.order);
         p.u = reinterpret_cast<uint16_t *>(ws + L.u);

@@ -423,7 +423,9 @@ typedef struct q4k_lora_task {
  * tasks (at most Q4K_MAX_TASKS).  Up to 64 columns take one launch and no
  * workspace (q4k_lora_workspace_bytes 0); more take three launches, whose
  * workspace need not be initialised (a wait that gives up after 2 s leaves
- * Q4K_ETIMEOUT in its status word, see q4k_workspace_status). */
+ * Q4K_ETIMEOUT in its status word, see q4k_workspace_status).  Of a workspace
+ * shared with the GEMV calls only that word of the control words changes, so
+ * q4k_gemv_batch_persistent needs no new q4k_workspace_init behind it. */
 Q4K_API size_t q4k_lora_workspace_bytes(const q4k_lora_task *tasks, int ntasks, int ncols);
 Q4K_API int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int32_t *ids, void *workspace,
                            size_t workspace_bytes, q4k_stream_t stream);
