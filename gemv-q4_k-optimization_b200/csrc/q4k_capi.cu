@@ -11,6 +11,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -54,14 +55,17 @@ int num_sms_or_bound() {
 
 // Workspace layout: [status word | pad][counters][partials][activations];
 // header bytes 4 (gather), 64 (dynamic tickets) and 128 (grid barrier) hold sync words.
+// The counters' room is the same for every call (up to 16384 row groups), so
+// that a call of few row groups does not put its partials where the next
+// single-launch call of more expects counters left at zero.
 struct Layout {
     size_t counters_off = 0, partials_off = 0, act_off = 0, total = 0;
 };
 
 Layout make_layout(int64_t n_rowgroups, int ncols, size_t act_bytes, int64_t partial_slots) {
     Layout L;
-    L.counters_off = kAlign;
-    L.partials_off = L.counters_off + round_up(static_cast<size_t>(n_rowgroups) * 4, kAlign);
+    L.counters_off = kHeaderBytes;
+    L.partials_off = std::max<size_t>(kControlBytes, L.counters_off + round_up(static_cast<size_t>(n_rowgroups) * 4, kAlign));
     L.act_off = L.partials_off + round_up(static_cast<size_t>(partial_slots) * ncols * 32 * sizeof(float), kAlign);
     L.total = L.act_off + round_up(act_bytes, kAlign);
     return L;

@@ -9,12 +9,13 @@
 // dst but no scratch buffer to pass as the workspace of q4k_mul_mat_vec.
 //
 // This entry point brings its own scratch: a file-scope device array of
-// kScratchBytes (4 MiB), which every GPU that loads the library holds until
-// the process exits.  It is one array per device, shared by every call of
-// this entry point on that device; each call starts by clearing the parts
-// that must start at zero (status word and split counters, done by the prep
-// kernel), so leftovers of the previous call do no harm, but two calls that
-// can overlap on the GPU (e.g. issued on two streams) race on it.
+// kScratchBytes (4 MiB; behind a workspace's control words), which every GPU
+// that loads the library holds until the process exits.  It is one array per
+// device, shared by every call of this entry point on that device; each call
+// starts by clearing the parts that must start at zero (status word and split
+// counters, done by the prep kernel), so leftovers of the previous call do no
+// harm, but two calls that can overlap on the GPU (e.g. issued on two
+// streams) race on it.
 #include "q4k_gemv.h"
 #include "q4k_internal.h"
 
@@ -25,10 +26,11 @@
 namespace {
 
 constexpr size_t kScratchBytes = size_t(4) << 20;  // 4 MiB per device
+constexpr size_t kArrayBytes = kScratchBytes + q4k::kControlBytes;
 
 // In host code this name is only a host-side stand-in for the device array;
 // kernels get its device address from cudaGetSymbolAddress (below).
-static __device__ __align__(256) unsigned char g_noalloc_scratch[kScratchBytes];
+static __device__ __align__(256) unsigned char g_noalloc_scratch[kArrayBytes];
 
 // Device address of the scratch array on the current device.  Looked up on
 // every call (the lookup allocates nothing and is cheap), so the address
@@ -64,12 +66,12 @@ int q4k_mul_mat_vec_noalloc(const void *W, const float *x, float *dst, int64_t K
         return q4k_mul_mat_vec(W, x, dst, K, nrows, ncols, stride_row_x, stride_col_x, stride_col_dst, nullptr, 0,
                                stream);
     }
-    if (need > kScratchBytes) {
+    if (need > kArrayBytes) {
         char msg[256];
         snprintf(msg, sizeof(msg),
                  "q4k_mul_mat_vec_noalloc: this call needs %zu bytes of scratch, more than the %zu-byte "
                  "built-in array (nrows=%lld K=%lld ncols=%d); use q4k_mul_mat_vec with a caller workspace",
-                 need, kScratchBytes, (long long)nrows, (long long)K, ncols);
+                 need, kArrayBytes, (long long)nrows, (long long)K, ncols);
         q4k::set_last_error_message(msg);
         return Q4K_EINVAL;
     }
@@ -83,7 +85,7 @@ int q4k_mul_mat_vec_noalloc(const void *W, const float *x, float *dst, int64_t K
         return Q4K_ECUDA;
     }
     return q4k_mul_mat_vec(W, x, dst, K, nrows, ncols, stride_row_x, stride_col_x, stride_col_dst, scratch,
-                           kScratchBytes, stream);
+                           kArrayBytes, stream);
 }
 
 }  // extern "C"

@@ -311,8 +311,9 @@ Q4K_API int q4k_gather_wait(const q4k_gather *gather, void *workspace, size_t wo
  * needs the same workspace size (q4k_batch_workspace_bytes) and its control
  * words in a known state on entry: zero the workspace once with
  * q4k_workspace_init before the first call; every call that completes leaves
- * them valid again (the two-launch calls may use the same workspace in
- * between).  After a call reports Q4K_ETIMEOUT (q4k_workspace_status) call
+ * them valid again (the other calls may use the same workspace in between,
+ * in launches of up to 524288 rows; a larger one needs q4k_workspace_init
+ * before the next single-launch call).  After a call reports Q4K_ETIMEOUT (q4k_workspace_status) call
  * q4k_workspace_init again.  gather may be NULL (no all-gather) or a
  * descriptor as for q4k_gemv_batch_allgather; the launch then waits for the
  * previous gathering call's rows before it reads its activations. */
@@ -359,8 +360,8 @@ Q4K_API int q4k_gemv_sharded(const void *W_shard, const float *x, float *y, int6
  * every buffer ahead and forbid cudaMalloc on the decode path, host
  * applications that own the GPU memory budget): the scratch comes from a
  * 4 MiB array built into the library, held on every GPU that loads it until
- * the process exits.  Calls that need more (q4k_gemv_workspace_bytes(nrows, K,
- * ncols) > q4k_noalloc_scratch_bytes()) return Q4K_EINVAL with a message.
+ * the process exits.  Calls that do not fit return Q4K_EINVAL with a message;
+ * q4k_gemv_workspace_bytes(nrows, K, ncols) <= q4k_noalloc_scratch_bytes() fits.
  * The first call on a device looks up the array's device address; make that
  * first call before any stream capture.  All calls on a device share the
  * array: calls that can overlap on the GPU (e.g. on two streams) race. */
@@ -368,7 +369,7 @@ Q4K_API int q4k_mul_mat_vec_noalloc(const void *W, const float *x, float *dst,
                                     int64_t K, int64_t nrows, int ncols,
                                     int64_t stride_row_x, int64_t stride_col_x, int64_t stride_col_dst,
                                     q4k_stream_t stream);
-/* Size of that built-in scratch array in bytes. */
+/* Size of that built-in scratch array in bytes (besides its control words). */
 Q4K_API size_t q4k_noalloc_scratch_bytes(void);
 
 /* ---- what each request of a batch brings of its own ----------------------------- */

@@ -45,3 +45,30 @@ def test_adapters_of_many_columns_between_single_launch_calls(q4k, step):
         for _ in range(2):
             assert same(run(ws), want)
     assert ws.ptr == ptr and ws.status() == 0 and np.prod(ws.buf.shape) == 1 << 24
+
+
+@pytest.mark.parametrize("rows,ncols", [(32, 8), (64, 3), (160, 2), (333, 1)])
+def test_smaller_calls_between_single_launch_calls(q4k, step, rows, ncols):
+    """Calls of fewer row groups, whose partial sums and activation records follow their own counters."""
+    import torch
+    run, want = step
+    ws = q4k.Workspace(1 << 24)
+    assert same(run(ws), want)
+    rng = np.random.default_rng(rows)
+    W = torch.from_numpy(q4k.gen_q4k_numpy(rng, rows, 14336)).cuda()
+    x = torch.from_numpy(rng.standard_normal((ncols, 14336)).astype(np.float32)).cuda()
+    alone = q4k.mul_mat_vec_q(W, x, ws=q4k.Workspace())
+    y = torch.empty_like(alone)
+    tasks = q4k.make_tasks([W], [x], [y])
+    for call in (lambda: q4k.mul_mat_vec_q(W, x, out=y, ws=ws), lambda: q4k.gemv_batch(tasks, ncols, ws),
+                 lambda: q4k.gemv_batch_persistent(tasks, ncols, ws)):
+        y.fill_(float("nan"))
+        call()
+        assert torch.equal(y, alone)
+        assert same(run(ws), want)
+    assert ws.status() == 0 and control_words_zero(ws, n_rowgroups(MISTRAL, 1))
+
+
+def test_counters_have_the_same_room_in_every_workspace(q4k):
+    """16384 row groups' counters behind the header, whatever the call."""
+    assert q4k.gemv_workspace_bytes(32, 256, 1) >= 256 + 16384 * 4
