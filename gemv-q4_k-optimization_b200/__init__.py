@@ -639,10 +639,17 @@ def make_lora_tasks(items: Sequence):
     """ctypes q4k_lora_task array for lora_batch from dicts with keys x (ncols, K) fp32,
     A (slots, rank, K) and B (slots, nrows, rank) of one type (fp32, fp16 or bf16), out
     (ncols, nrows) and optionally base (fp32 like out, may be out itself), ranks (slots
-    int32) and scales (slots fp32).  The tensors must outlive the array."""
+    int32) and scales (slots fp32).  The tensors must outlive the array, which keeps
+    their number of columns and their device for lora_batch's checks."""
     if any(it.get("out") is None for it in items):
         raise Q4KError(1, "make_lora_tasks: an item has no out")
-    return (LoraTask * len(items)).from_buffer_copy(_native().lora_pack(items))
+    arr = (LoraTask * len(items)).from_buffer_copy(_native().lora_pack(items))
+    if len(items):
+        x = items[0]["x"]
+        arr.ncols, arr.device = x.shape[0] if x.dim() == 2 else 1, x.get_device()
+    else:
+        arr.ncols, arr.device = 0, -1
+    return arr
 
 
 def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
@@ -652,7 +659,9 @@ def lora_batch(tasks, ids, ws: Workspace | None = None, stream=None):
     adapter, out[j] = base[j]).  tasks: dicts as for make_lora_tasks (out may be left
     out), returns the list of outputs; or its array, returns None."""
     if isinstance(tasks, ctypes.Array):
-        return _native().lora_run(tasks, ids, ws, _handle(stream))
+        if tasks._type_ is not LoraTask or not hasattr(tasks, "ncols"):
+            raise Q4KError(1, f"lora_batch: an array from make_lora_tasks expected, not {type(tasks).__name__}")
+        return _native().lora_run(tasks, ids, ws, _handle(stream), tasks.ncols, tasks.device)
     return _native().lora_batch(tasks, ids, ws, _handle(stream))
 
 

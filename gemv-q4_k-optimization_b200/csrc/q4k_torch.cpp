@@ -329,21 +329,26 @@ PyObject *py_lora_pack(PyObject *, PyObject *const *v, Py_ssize_t n) {
     });
 }
 
-// lora_run(tasks' bytes (buffer), ids, ws, stream)
+// lora_run(tasks' bytes (buffer), ids, ws, stream, the tasks' columns, their device)
 PyObject *py_lora_run(PyObject *, PyObject *const *v, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
-        if (n != 4) refuse("lora_run: 4 arguments");
+        if (n != 6) refuse("lora_run: 6 arguments");
+        const int64_t ncols = PyLong_AsLongLong(v[4]), device = PyLong_AsLongLong(v[5]);
+        if (PyErr_Occurred()) throw PythonError{};
         Py_buffer buf;
         if (PyObject_GetBuffer(v[0], &buf, PyBUF_SIMPLE) != 0) throw PythonError{};
         struct Release {
             Py_buffer *b;
             ~Release() { PyBuffer_Release(b); }
         } release{&buf};
-        const at::Tensor &ids = tensor(v[1], "ids");
-        const int dev = device_of(ids, "ids");
+        const Py_ssize_t count = buf.len / static_cast<Py_ssize_t>(sizeof(q4k_lora_task));
+        if (buf.len % static_cast<Py_ssize_t>(sizeof(q4k_lora_task)) != 0 || count > Q4K_MAX_TASKS)
+            refuse("tasks: %lld bytes are not up to %d tasks", (long long)buf.len, Q4K_MAX_TASKS);
+        if (count == 0) Py_RETURN_NONE;
+        const int dev = device_of(tensor(v[1], "ids"), "ids");
+        if (dev != device) refuse("ids: on cuda:%d, the tasks' tensors are on cuda:%lld", dev, (long long)device);
         Where where(dev, v[3]);
-        run_tasks(static_cast<const q4k_lora_task *>(buf.buf), static_cast<int>(buf.len / sizeof(q4k_lora_task)),
-                  ids.dim() == 1 ? ids.size(0) : 0, dev, v[1], v[2], where);
+        run_tasks(static_cast<const q4k_lora_task *>(buf.buf), static_cast<int>(count), ncols, dev, v[1], v[2], where);
         Py_RETURN_NONE;
     });
 }

@@ -353,3 +353,18 @@ def test_lora_refusals_of_the_wrapper(q4k):
                dict(A=d["A"].transpose(1, 2)), dict(x=d["x"].cpu()), dict(ids=d["ids"].cpu()), dict(out=d["x"][:, :32])):
         with pytest.raises(q4k.Q4KError):
             q4k.lora_add(**{**ok, **kw})
+
+
+@pytest.mark.parametrize("ncols", [8, 100])
+def test_lora_task_array_wants_its_own_number_of_columns(q4k, ncols):
+    """More or fewer ids than the tensors behind a task array have columns are refused, and nothing is written."""
+    import torch
+    d = make(4, ncols, 64, 32, 2, 4, "float16")
+    out = torch.full_like(d["base"], 7.0)
+    arr = q4k.make_lora_tasks([dict(x=d["x"], A=d["A"], B=d["B"], ranks=d["ranks"], scales=d["scales"], base=d["base"], out=out)])
+    for ids in (torch.cat([d["ids"], d["ids"]]), d["ids"][:-1], d["ids"][:0], d["ids"].cpu(), d["ids"].long(), d["ids"][None], None):
+        with pytest.raises(q4k.Q4KError):
+            q4k.lora_batch(arr, ids)
+    assert (out == 7).all()
+    q4k.lora_batch(arr, d["ids"])
+    check_exact(out, reference(d))

@@ -154,3 +154,15 @@ def test_structures_match_the_header(q4k):
     with pytest.raises(q4k.Q4KError):
         q4k.lora_batch([dict(x=torch.zeros(1, 8))], torch.zeros(1, dtype=torch.int32))
     assert q4k.lora_batch([], torch.zeros(1, dtype=torch.int32)) == []
+
+
+def test_lora_batch_takes_no_other_array(q4k):
+    """Arrays of GEMV tasks, and adapter tasks whose number of columns nobody checked, are refused."""
+    import torch
+    ids = torch.zeros(1, dtype=torch.int32)
+    for arr in ((q4k.Task * 2)(), (q4k.TaskEx * 1)(), (ctypes.c_char * 144)(), (q4k.LoraTask * 1)()):
+        with pytest.raises(q4k.Q4KError, match="make_lora_tasks"):
+            q4k.lora_batch(arr, ids)
+    with pytest.raises(q4k.Q4KError, match="bytes"):  # not a whole number of tasks
+        q4k._native().lora_run(bytes(ctypes.sizeof(q4k.LoraTask) + 8), ids, None, None, 1, 0)
+    assert q4k.lora_batch(q4k.make_lora_tasks([]), ids) is None
