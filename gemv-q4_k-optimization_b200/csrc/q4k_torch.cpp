@@ -234,7 +234,7 @@ PyObject *add_task(LoraCall &c, std::optional<Where> &where, PyObject *stream, P
 
 // The call itself: ids, and a workspace where the library wants one (ws None:
 // scratch of this call's own, so that calls on several streams or in several
-// graphs share nothing; else an object with ensure(bytes), ptr and nbytes).
+// graphs share nothing; else a Workspace: ensure(bytes) and buf, a tensor on the tasks' device).
 void run_tasks(const q4k_lora_task *tasks, int n, int64_t ncols, int device, PyObject *ids, PyObject *ws, const Where &where) {
     const int32_t *idp = flat<int32_t>(ids, "ids", at::kInt, ncols, device);
     if (idp == nullptr && ncols > 0) refuse("ids: %lld device ints expected", (long long)ncols);
@@ -249,11 +249,13 @@ void run_tasks(const q4k_lora_task *tasks, int n, int64_t ncols, int device, PyO
             PyObject *r = PyObject_CallMethod(ws, "ensure", "n", static_cast<Py_ssize_t>(need));
             if (r == nullptr) throw PythonError{};
             Py_DECREF(r);
-            PyObject *q = PyObject_GetAttrString(ws, "ptr");
-            if (q == nullptr) throw PythonError{};
-            p = PyLong_AsVoidPtr(q);
-            Py_DECREF(q);
-            if (PyErr_Occurred()) throw PythonError{};
+            Refs hold;
+            if ((hold.v[0] = PyObject_GetAttrString(ws, "buf")) == nullptr) throw PythonError{};
+            hold.n = 1;
+            const at::Tensor &buf = tensor(hold.v[0], "ws.buf");
+            if (!buf.is_cuda() || buf.get_device() != device)
+                refuse("ws: a workspace on cuda:%d expected, got %s", device, shape_of(buf).c_str());
+            p = buf.data_ptr();
         }
     }
     check(g_lora(tasks, n, static_cast<int>(ncols), idp, p, need, where.stream));

@@ -368,3 +368,12 @@ def test_lora_task_array_wants_its_own_number_of_columns(q4k, ncols):
     assert (out == 7).all()
     q4k.lora_batch(arr, d["ids"])
     check_exact(out, reference(d))
+
+
+def test_lora_workspace_of_another_device_is_refused(q4k):
+    import torch
+    d = make(4, 100, 64, 32, 2, 4, "float16")
+    with pytest.raises(q4k.Q4KError, match="workspace"):
+        q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], ws=q4k.Workspace(1 << 20, device="cpu"))
+    got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], ranks=d["ranks"], scales=d["scales"], ws=q4k.Workspace(0, device="cuda"))
+    check_exact(got, reference(d, use_base=False))
