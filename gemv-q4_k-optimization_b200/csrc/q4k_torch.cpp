@@ -414,15 +414,17 @@ PyObject *py_rope(PyObject *, PyObject *const *v, Py_ssize_t n) {
             axes = static_cast<int>(PySequence_Fast_GET_SIZE(s));
             if (axes < 1 || axes > Q4K_MAX_ROPE_AXES) refuse("1 to %d sections expected", Q4K_MAX_ROPE_AXES);
             for (int i = 0; i < axes; ++i) {
-                sections[i] = static_cast<int>(PyLong_AsLong(PySequence_Fast_GET_ITEM(s, i)));
-                if (PyErr_Occurred()) throw PythonError{};
+                const long v = PyLong_AsLong(PySequence_Fast_GET_ITEM(s, i));
+                if (v == -1 && PyErr_Occurred()) throw PythonError{};
+                if (v < 0 || v > Q4K_MAX_ROPE_DIM) refuse("sections[%d]=%ld outside 0..%d", i, v, Q4K_MAX_ROPE_DIM);
+                sections[i] = static_cast<int>(v);
             }
         }
         const at::Tensor &pos = dense(v[1], "pos", 2, dev, at::kInt);
         if (pos.size(0) != axes || pos.size(1) != ncols)
             refuse("pos %s: (%d, %lld) expected", shape_of(pos).c_str(), axes, (long long)ncols);
         const int64_t half = tensor(v[2], "inv_freq").numel();
-        if (half > Q4K_MAX_ROPE_DIM) refuse("inv_freq: at most %d values", Q4K_MAX_ROPE_DIM / 2);
+        if (half > Q4K_MAX_ROPE_DIM / 2) refuse("inv_freq: at most %d values", Q4K_MAX_ROPE_DIM / 2);
         const double *inv = flat<double>(v[2], "inv_freq", at::kDouble, half, dev);
         const int layout = static_cast<int>(PyLong_AsLong(v[4])), order = static_cast<int>(PyLong_AsLong(v[5]));
         const double scale = PyFloat_AsDouble(v[6]);

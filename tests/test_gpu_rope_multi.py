@@ -195,3 +195,12 @@ def test_rope_empty_and_refused_calls(q4k):
                dict(inv_freq=q4k.rope_inv_freq(66)), dict(x=[x, x], out=[x, x])):
         with pytest.raises(q4k.Q4KError):
             q4k.rope_multi(**{**ok, **kw})
+
+
+def test_rope_sections_of_more_than_an_int_are_refused(q4k):
+    """2^32 + 16 is not taken for 16 (nor 2^32 - 1 for -1)."""
+    import torch
+    x, p = torch.randn(3, 2, 64, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for sections in ((2**32 + 16, 16), (16, 2**32 + 16), (2**32 - 1, 32), (-1, 33), (1025, 1), (2**70, 1)):
+        with pytest.raises((q4k.Q4KError, OverflowError)):
+            q4k.rope_multi(x, p, q4k.rope_inv_freq(64), sections)
