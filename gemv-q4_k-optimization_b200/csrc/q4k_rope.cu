@@ -5,7 +5,8 @@
 //   (x_a, x_b) -> scale * (x_a cos - x_b sin, x_b cos + x_a sin).
 // The angle is formed in fp64 as a number of half turns and reduced there
 // (a far position times an inverse frequency holds more digits than fp32
-// keeps); its sine and cosine are fp32.
+// keeps). Its sine and cosine are fp32: those of the angle's fp32 part, turned
+// by the remainder (at most 2^-25 half turns, so its first power is enough).
 #include "q4k_device.cuh"
 #include "q4k_request.h"
 
@@ -54,9 +55,11 @@ __device__ __forceinline__ float2 turn_of(const RopeParams &P, int i, int64_t j)
     const double turns = static_cast<double>(P.pos[axis_of(P, i) * P.sp_axis + j]) * P.inv_freq[i] *
                          0.31830988618379067154;  // 1/pi: half turns
     const double r = turns - 2.0 * rint(0.5 * turns);
+    const float near = static_cast<float>(r);
+    const float left = static_cast<float>((r - static_cast<double>(near)) * 3.14159265358979323846);
     float s, c;
-    sincospif(static_cast<float>(r), &s, &c);
-    return make_float2(c * P.scale, s * P.scale);
+    sincospif(near, &s, &c);
+    return make_float2(fmaf(-s, left, c) * P.scale, fmaf(c, left, s) * P.scale);
 }
 
 constexpr int kThreads = 256;

@@ -204,3 +204,25 @@ def test_rope_sections_of_more_than_an_int_are_refused(q4k):
     for sections in ((2**32 + 16, 16), (16, 2**32 + 16), (2**32 - 1, 32), (-1, 33), (1025, 1), (2**70, 1)):
         with pytest.raises((q4k.Q4KError, OverflowError)):
             q4k.rope_multi(x, p, q4k.rope_inv_freq(64), sections)
+
+
+@pytest.mark.parametrize("layout", ["half", "adjacent"])
+@pytest.mark.parametrize("ncols", [40, 700])
+@pytest.mark.parametrize("base", [1e4, 1e6])
+def test_rope_sines_and_cosines_hold_their_digits(q4k, layout, ncols, base):
+    """Pairs (1, 0) give the cosine and the sine themselves, so small ones show an angle that was rounded to fp32
+    (up to 2^-25 half turns, 9.4e-8, whatever the sine). Tolerance: one ulp of sincospif, half of one for the
+    remainder's addition (a value's ulp is at most 2^-23 of it; 2 in all for a result in the next binade); the
+    remainder's rounding and second power are below 1e-14, the fp64 product's two roundings at 1600 half turns
+    1600 * 2^-52 * pi = 1.2e-12."""
+    import torch
+    rng = np.random.default_rng(ncols)
+    half = 64
+    x = np.zeros((ncols, 2, 2 * half), np.float32)
+    x[..., :half if layout == "half" else None:1 if layout == "half" else 2] = 1.0
+    pos = rng.integers(0, 5000, (1, ncols)).astype(np.int32)
+    inv = q4k.rope_inv_freq(2 * half, base)
+    got = q4k.rope_multi(torch.from_numpy(x).cuda(), torch.from_numpy(pos).cuda(), inv, (half,), layout=layout)
+    want, _ = reference(x, pos, inv.cpu().numpy(), (half,), layout, "blocks", 1.0)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert (err <= 2 * 2.0 ** -23 * np.abs(want) + 2e-12).all(), (err / (2.0 ** -23 * np.abs(want) + 1e-12)).max()
