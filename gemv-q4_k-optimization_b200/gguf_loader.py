@@ -83,15 +83,20 @@ class GGUFModel:
         """Keyword arguments for q4k.rope_multi (inv_freq, sections, layout, order) from the
         metadata `<arch>.rope.*` and the `rope_freqs.weight` factors.  Sections are the
         M-RoPE `dimension_sections` without trailing zeros (one axis where there are none).
+        Without a `dimension_count` heads turn whole: `attention.key_length` values, else
+        the embedding's share of a head.
         layout: "adjacent" for llama files (their q and k rows are stored for neighbouring
         pairs), else "half", unless given."""
         a = self.arch
         n_rot = self.field(f"{a}.rope.dimension_count")
+        if n_rot is None:  # whole heads
+            n_rot = self.field(f"{a}.attention.key_length")
         if n_rot is None:
-            heads, width = self.field(f"{a}.attention.head_count"), self.field(f"{a}.embedding_length")
-            if not heads or not width:
-                raise KeyError(f"{self.path}: no {a}.rope.dimension_count")
-            n_rot = int(width) // int(heads)
+            heads = set(self.array(f"{a}.attention.head_count") or [])  # one number, or one per layer
+            width = self.field(f"{a}.embedding_length")
+            if len(heads) != 1 or 0 in heads or not width:
+                raise KeyError(f"{self.path}: no {a}.rope.dimension_count, nor the width of a head")
+            n_rot = int(width) // int(heads.pop())
         base = self.field(f"{a}.rope.freq_base") or 10000.0
         factor = self.field(f"{a}.rope.scaling.factor")
         linear = self.field(f"{a}.rope.scaling.type") == "linear"

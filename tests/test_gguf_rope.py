@@ -1,0 +1,42 @@
+"""Rotary parameters read from a model file's metadata (GGUFModel.rope): what the file
+asks for is given, and what it asks for that cannot be given is refused."""
+from __future__ import annotations
+
+import importlib
+
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def loader(q4k):
+    return importlib.import_module("q4k_b200.gguf_loader")
+
+
+@pytest.fixture
+def rope(q4k, loader, tmp_path):
+    """rope(arch, metadata without the architecture's prefix, ...) of a file with that metadata."""
+    def read(arch, meta, extra=None, **kw):
+        loader.write_q4k_gguf(tmp_path / "m.gguf", {}, arch=arch, extra_f32=extra or {"t": np.ones(4, np.float32)},
+                              metadata={f"{arch}.{k}": v for k, v in meta.items()})
+        return loader.GGUFModel(tmp_path / "m.gguf").rope(q4k, device="cpu", **kw)
+    return read
+
+
+def freqs(n_rot, base=10000.0):
+    return base ** (-np.arange(n_rot // 2) * 2.0 / n_rot)
+
+
+def test_rotated_width(rope):
+    """The file's count of rotated values, else the length of its keys, else its embedding's share per head."""
+    heads = {"embedding_length": 1024, "attention.head_count": 32}
+    for meta, want in (({**heads}, 32), ({**heads, "attention.key_length": 128}, 128),
+                       ({**heads, "attention.key_length": 128, "rope.dimension_count": 64}, 64),
+                       ({"attention.key_length": 80}, 80),
+                       ({"embedding_length": 1024, "attention.head_count": [16, 16]}, 64)):
+        p = rope("llama", meta)
+        assert np.allclose(p["inv_freq"].numpy(), freqs(want), rtol=1e-14) and p["sections"] == (want // 2,)
+    for meta in ({}, {"embedding_length": 1024}, {"embedding_length": 1024, "attention.head_count": [16, 8]},
+                 {"embedding_length": 1024, "attention.head_count": 0}):
+        with pytest.raises(KeyError):
+            rope("llama", meta)
