@@ -84,7 +84,9 @@ class GGUFModel:
         metadata `<arch>.rope.*` and the `rope_freqs.weight` factors.  Sections are the
         M-RoPE `dimension_sections` without trailing zeros (one axis where there are none).
         Without a `dimension_count` heads turn whole: `attention.key_length` values, else
-        the embedding's share of a head.
+        the embedding's share of a head.  A `scaling.factor` divides the frequencies unless
+        the file's `scaling.type` is none; files that ask for another scaling (yarn,
+        longrope) or for a second set of frequencies are refused.
         layout: "adjacent" for llama files (their q and k rows are stored for neighbouring
         pairs), else "half", unless given."""
         a = self.arch
@@ -98,9 +100,19 @@ class GGUFModel:
                 raise KeyError(f"{self.path}: no {a}.rope.dimension_count, nor the width of a head")
             n_rot = int(width) // int(heads.pop())
         base = self.field(f"{a}.rope.freq_base") or 10000.0
-        factor = self.field(f"{a}.rope.scaling.factor")
-        linear = self.field(f"{a}.rope.scaling.type") == "linear"
-        scale = 1.0 / factor if linear and factor else 1.0
+        kind = self.field(f"{a}.rope.scaling.type") or "linear"
+        if kind not in ("linear", "none"):
+            raise ValueError(f"{self.path}: rotary scaling {kind!r} (only linear scaling and none)")
+        # other frequencies for long contexts or for windowed layers, or a factor on the turned values
+        for key, same in (("rope.scaling.attn_factor", 1.0), ("rope.scaling.alpha", 0.0), ("rope.freq_base_swa", base),
+                          ("rope.dimension_count_swa", n_rot)):
+            v = self.field(f"{a}.{key}")
+            if v is not None and v != same:
+                raise ValueError(f"{self.path}: {a}.{key} = {v} is not supported")
+        if "rope_factors_long.weight" in self.tensors or "rope_factors_short.weight" in self.tensors:
+            raise ValueError(f"{self.path}: rotary factors by context length are not supported")
+        factor = self.field(f"{a}.rope.scaling.factor") or self.field(f"{a}.rope.scale_linear")
+        scale = 1.0 / factor if kind == "linear" and factor else 1.0
         t = self.tensors.get("rope_freqs.weight")
         sections = [int(v) for v in self.array(f"{a}.rope.dimension_sections") or []]
         while sections and sections[-1] == 0:

@@ -40,3 +40,23 @@ def test_rotated_width(rope):
                  {"embedding_length": 1024, "attention.head_count": 0}):
         with pytest.raises(KeyError):
             rope("llama", meta)
+
+
+def test_scaling(rope):
+    """A factor without a type is linear, type none scales nothing, and what is not a factor on the frequencies is refused."""
+    d = {"rope.dimension_count": 64, "rope.freq_base": 50000.0}
+    for meta, by in (({}, 1.0), ({"rope.scaling.type": "linear", "rope.scaling.factor": 4.0}, 4.0), ({"rope.scaling.factor": 4.0}, 4.0),
+                     ({"rope.scaling.type": "none", "rope.scaling.factor": 4.0}, 1.0), ({"rope.scaling.type": "linear"}, 1.0),
+                     ({"rope.scaling.factor": 0.0}, 1.0), ({"rope.scale_linear": 2.0}, 2.0), ({"rope.scaling.attn_factor": 1.0}, 1.0),
+                     ({"rope.freq_base_swa": 50000.0}, 1.0)):
+        assert np.allclose(rope("llama", {**d, **meta})["inv_freq"].numpy(), freqs(64, 50000.0) / by, rtol=1e-14), meta
+    for meta in ({"rope.scaling.type": "yarn", "rope.scaling.factor": 4.0}, {"rope.scaling.type": "yarn"},
+                 {"rope.scaling.type": "longrope"}, {"rope.scaling.attn_factor": 1.2}, {"rope.freq_base_swa": 10000.0},
+                 {"rope.dimension_count_swa": 32}, {"rope.scaling.alpha": 1000.0}):
+        with pytest.raises(ValueError):
+            rope("llama", {**d, **meta})
+    with pytest.raises(ValueError):
+        rope("llama", d, extra={"rope_factors_long.weight": np.ones(32, np.float32), "rope_factors_short.weight": np.ones(32, np.float32)})
+    f = np.linspace(1, 8, 32, dtype=np.float32)
+    p = rope("llama", {**d, "rope.scaling.factor": 2.0}, extra={"rope_freqs.weight": f})
+    assert np.allclose(p["inv_freq"].numpy(), freqs(64, 50000.0) / 2 / f.astype(np.float64), rtol=1e-14)
