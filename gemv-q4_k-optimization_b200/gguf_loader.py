@@ -30,6 +30,17 @@ LLAMA_LAYER = (("q", "attn_q", "attn"), ("k", "attn_k", "attn"), ("v", "attn_v",
                ("o", "attn_output", "o"), ("gate", "ffn_gate", "ffn"), ("up", "ffn_up", "ffn"),
                ("down", "ffn_down", "down"))
 
+# How an architecture's files store the rotated pairs of q and k (neighbours, or
+# halves of the rotated width), and how it deals its pairs out to several axes.
+ROPE_LAYOUTS = {
+    **dict.fromkeys(("llama", "baichuan", "command-r", "cohere2", "deepseek", "granite", "granitemoe", "internlm2",
+                     "minicpm", "olmo", "smollm3", "xverse"), "adjacent"),
+    **dict.fromkeys(("exaone", "falcon", "gemma", "gemma2", "gptneox", "nemotron", "olmo2", "olmoe", "orion", "phi2", "phi3",
+                     "qwen2", "qwen2moe", "qwen2vl", "qwen3", "qwen3moe", "qwen3vl", "qwen3vlmoe", "stablelm",
+                     "starcoder2"), "half"),
+}
+ROPE_ORDERS = {"llama": "blocks", "qwen2vl": "blocks", "qwen3vl": "interleaved", "qwen3vlmoe": "interleaved"}
+
 
 @dataclass
 class Q4KTensor:
@@ -79,16 +90,16 @@ class GGUFModel:
             return None
         return [v for i in f.data for v in np.asarray(f.parts[i]).tolist()]
 
-    def rope(self, q4k, layout: str | None = None, order: str = "blocks", device="cuda") -> dict:
+    def rope(self, q4k, layout: str | None = None, order: str | None = None, device="cuda") -> dict:
         """Keyword arguments for q4k.rope_multi (inv_freq, sections, layout, order) from the
         metadata `<arch>.rope.*` and the `rope_freqs.weight` factors.  Sections are the
         M-RoPE `dimension_sections` without trailing zeros (one axis where there are none).
         Without a `dimension_count` heads turn whole: `attention.key_length` values, else
         the embedding's share of a head.  A `scaling.factor` divides the frequencies unless
         the file's `scaling.type` is none; files that ask for another scaling (yarn,
-        longrope) or for a second set of frequencies are refused.
-        layout: "adjacent" for llama files (their q and k rows are stored for neighbouring
-        pairs), else "half", unless given."""
+        longrope) or for a second set of frequencies are refused.  layout, and order where
+        there are several axes, have to be given for an architecture that ROPE_LAYOUTS and
+        ROPE_ORDERS do not know."""
         a = self.arch
         n_rot = self.field(f"{a}.rope.dimension_count")
         if n_rot is None:  # whole heads
@@ -117,9 +128,13 @@ class GGUFModel:
         sections = [int(v) for v in self.array(f"{a}.rope.dimension_sections") or []]
         while sections and sections[-1] == 0:
             sections.pop()
+        layout = layout or ROPE_LAYOUTS.get(a)
+        order = order or (ROPE_ORDERS.get(a) if len(sections) > 1 else "blocks")
+        if layout is None or order is None:
+            raise ValueError(f"{self.path}: architecture {a!r}: give the rotary {'order' if layout else 'layout'}")
         return dict(inv_freq=q4k.rope_inv_freq(int(n_rot), base, scale, None if t is None else np.array(t.data), device=device),
                     sections=tuple(sections) or (int(n_rot) // 2,),
-                    layout=layout or ("adjacent" if a == "llama" else "half"), order=order)
+                    layout=layout, order=order)
 
     # ---- tensors ----------------------------------------------------------
     def q4k(self, name: str) -> Q4KTensor:

@@ -60,3 +60,29 @@ def test_scaling(rope):
     f = np.linspace(1, 8, 32, dtype=np.float32)
     p = rope("llama", {**d, "rope.scaling.factor": 2.0}, extra={"rope_freqs.weight": f})
     assert np.allclose(p["inv_freq"].numpy(), freqs(64, 50000.0) / 2 / f.astype(np.float64), rtol=1e-14)
+
+
+@pytest.mark.parametrize("arch,layout,order", [("llama", "adjacent", "blocks"), ("command-r", "adjacent", None), ("qwen2", "half", None),
+                                               ("qwen2vl", "half", "blocks"), ("qwen3vl", "half", "interleaved")])
+def test_layout_and_order_of_known_architectures(rope, arch, layout, order):
+    one = rope(arch, {"rope.dimension_count": 64})
+    assert (one["layout"], one["sections"], one["order"]) == (layout, (32,), "blocks")
+    several = {"rope.dimension_count": 64, "rope.dimension_sections": [12, 10, 10, 0]}
+    if order is None:
+        with pytest.raises(ValueError, match="order"):
+            rope(arch, several)
+    else:
+        p = rope(arch, several)
+        assert (p["layout"], p["sections"], p["order"]) == (layout, (12, 10, 10), order)
+    p = rope(arch, several, layout="half", order="interleaved")
+    assert (p["layout"], p["order"]) == ("half", "interleaved")
+
+
+def test_unknown_architectures_are_refused_unless_named(rope):
+    d = {"rope.dimension_count": 64}
+    with pytest.raises(ValueError, match="layout"):
+        rope("somethingnew", d)
+    assert rope("somethingnew", d, layout="adjacent")["layout"] == "adjacent"
+    with pytest.raises(ValueError, match="order"):
+        rope("somethingnew", {**d, "rope.dimension_sections": [20, 12]}, layout="half")
+    assert rope("somethingnew", {**d, "rope.dimension_sections": [20, 12]}, layout="half", order="blocks")["sections"] == (20, 12)
