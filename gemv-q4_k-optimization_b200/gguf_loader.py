@@ -203,14 +203,16 @@ def load_adapters(paths, names, device="cuda", dtype=None, strengths=None) -> di
     """Adapter files (llama.cpp's `adapter.type = lora`: `<tensor>.lora_a` with ne = [K, rank],
     `<tensor>.lora_b` with ne = [rank, rows]) stacked into slots, slot s = paths[s], for the
     matrices `names` (e.g. "blk.0.attn_q.weight"): name -> dict(A, B, ranks, scales) as
-    q4k.lora_batch takes them, in `dtype` (default: fp16).  The scale of a slot is
+    q4k.lora_batch takes them.  dtype: by default the files' own where all of these
+    matrices are fp16 or all bf16, else fp32; values that are finite in the file and not in
+    a given dtype are refused.  The scale of a slot is
     strengths[s] * alpha / rank (strengths[s] where the file's alpha is 0 or missing); a
     matrix that a file does not adapt has rank 0 in its slot; ranks are padded to a
     multiple of 8 so that rows stay 16-byte aligned.  Matrices that no file adapts are
     left out."""
     import gguf
     import torch
-    dtype = torch.float16 if dtype is None else dtype
+    names = list(names)
     files = []
     for path in paths:
         m = GGUFModel(path)
@@ -227,6 +229,19 @@ def load_adapters(paths, names, device="cuda", dtype=None, strengths=None) -> di
         else:  # bf16 and quantized adapters
             a = gguf.quants.dequantize(np.asarray(t.data), t.tensor_type)
         return np.ascontiguousarray(a.reshape([int(d) for d in t.shape][::-1][-2:]))
+
+    if dtype is None:  # one for all: a launch takes adapters of one type
+        Q = gguf.GGMLQuantizationType
+        kinds = {m.tensors[key].tensor_type for m, _ in files for name in names
+                 for key in (name + ".lora_a", name + ".lora_b") if key in m.tensors}
+        dtype = torch.float16 if kinds == {Q.F16} else torch.bfloat16 if kinds == {Q.BF16} else torch.float32
+
+    def converted(a: np.ndarray, path, name: str):
+        t = torch.from_numpy(a)
+        c = t.to(dtype)
+        if not torch.equal(torch.isfinite(c), torch.isfinite(t)):
+            raise OverflowError(f"{path}: {name}: values beyond {dtype}")
+        return c
 
     out = {}
     for name in names:
@@ -250,7 +265,7 @@ def load_adapters(paths, names, device="cuda", dtype=None, strengths=None) -> di
             if p is None:
                 continue
             r = p[0].shape[0]
-            A[s, :r], B[s, :, :r] = torch.from_numpy(p[0]).to(dtype), torch.from_numpy(p[1]).to(dtype)
+            A[s, :r], B[s, :, :r] = (converted(a, files[s][0].path, name) for a in p)
             ranks[s] = r
             scales[s] = strengths[s] * (files[s][1] / r if files[s][1] and r else 1.0)
         out[name] = dict(A=A.to(device), B=B.to(device), ranks=ranks.to(device), scales=scales.to(device))
