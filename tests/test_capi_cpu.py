@@ -229,3 +229,13 @@ def test_sharded_argument_checks(q4k):
     assert call(ws=None) == EWORKSPACE
     assert call(wsb=64) == EWORKSPACE
     assert call(ws=4096 + 16) == EWORKSPACE  # not 256-byte aligned
+
+
+def test_make_without_torch_builds_the_c_libraries(q4k):
+    """A Python without torch (here: no Python at all) skips the native front-end with a message; make succeeds."""
+    import subprocess
+    before = (q4k.HERE / "_q4k_torch.so").stat().st_mtime_ns
+    r = subprocess.run(["make", "-C", str(q4k.HERE), "PYTHON=false", "-W", "csrc/q4k_torch.cpp", "_q4k_torch.so"],
+                       capture_output=True, text=True)
+    assert r.returncode == 0 and "skipped" in r.stdout and "torch" in r.stdout, r.stdout + r.stderr
+    assert (q4k.HERE / "_q4k_torch.so").stat().st_mtime_ns == before
