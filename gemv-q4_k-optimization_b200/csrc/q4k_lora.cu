@@ -387,6 +387,26 @@ template <int N> __device__ __forceinline__ void pieces(float a, float b, uint32
         b = rest(b);
     }
 }
+// An infinity cut into pieces becomes inf, NaN, NaN, and times another's zero piece NaN. So what the MMAs give as
+// infinite or NaN is summed anew from the values themselves: it comes out as the fp32 sum, as with few columns.
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+template <typename T> __device__ __noinline__ float plain_dot(const T *a, const float *x, int K) {
+    float s = 0.0f;
+    for (int k = 0; k < K; ++k) s = fmaf(to_f32(a[k]), x[k], s);
+    return s;
+}
+template <typename T> __device__ __noinline__ float plain_sum(const T *b, const uint16_t *u, int64_t piece, int r) {
+    auto value = [&](int64_t i) { return __uint_as_float(static_cast<uint32_t>(u[i]) << 16); };
+    float s = 0.0f;
+    for (int k = 0; k < r; ++k) s = fmaf(to_f32(b[k]), value(k) + (value(piece + k) + value(2 * piece + k)), s);
+    return s;
+}
+// Pieces that add up to any value: the first holds what is not finite.
+__device__ __noinline__ void whole_pieces(float a, float b, uint32_t (&p)[3]) {
+    pieces(finite(a) ? a : 0.0f, finite(b) ? b : 0.0f, p);
+    if (!finite(a)) p[0] = (p[0] & 0xffff0000u) | (a != a ? 0x7fffu : __float_as_uint(a) >> 16);
+    if (!finite(b)) p[0] = (p[0] & 0xffffu) | (b != b ? 0x7fff0000u : __float_as_uint(b));
+}
 template <typename T> struct Weight;  // bf16 pieces of a weight
 template <> struct Weight<__nv_bfloat16> { static constexpr int kPieces = 1; };
 template <> struct Weight<__half> { static constexpr int kPieces = 2; };
@@ -661,8 +681,16 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
             v.x += w0.x + w1.x;
             v.y += w0.y + w1.y;
         }
+        const bool one = 2 * k < nr, two = 2 * k + 1 < nr;
+        float2 w = make_float2(one ? v.x * scale : 0.0f, two ? v.y * scale : 0.0f);
         uint32_t p[3];
-        pieces(2 * k < nr ? v.x * scale : 0.0f, 2 * k + 1 < nr ? v.y * scale : 0.0f, p);
+        if (fmaf(w.x, 0.0f, w.y * 0.0f) == 0.0f) {
+            pieces(w.x, w.y, p);
+        } else {
+            if (one && !finite(v.x)) w.x = plain_dot(A + 2 * k * t.sa_row, xcol[col], t.K) * scale;
+            if (two && !finite(v.y)) w.y = plain_dot(A + (2 * k + 1) * t.sa_row, xcol[col], t.K) * scale;
+            whole_pieces(w.x, w.y, p);
+        }
 #pragma unroll
         for (int e = 0; e < 3; ++e)
             *reinterpret_cast<uint32_t *>(P.u + (static_cast<int64_t>(e) * P.ncols + tile.first + col) * P.u_cols + t.u_off + r0 +
@@ -846,9 +874,30 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
             uint32_t v[16];
             __syncwarp();
             load_tmem(v, d + ((warp & 3) * 32 << 16) + c0 + 16 * h);
+            float probe = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (c0 + 16 * h + e < tile.count && n < n1) col[c0 + 16 * h + e].dst[n] = y[e] + __uint_as_float(v[e]);
+            for (int e = 0; e < 16; ++e) probe = fmaf(__uint_as_float(v[e]), 0.0f, probe);
+            if (probe == 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (c0 + 16 * h + e < tile.count && n < n1) col[c0 + 16 * h + e].dst[n] = y[e] + __uint_as_float(v[e]);
+                if (h == 0) ask(c0 + 16);
+                continue;
+            }
+            uint32_t anew = 0u;  // columns whose sum is not finite
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bool ok = finite(__uint_as_float(v[e]));
+                if (!ok) anew |= 1u << e;
+                if (ok && c0 + 16 * h + e < tile.count && n < n1) col[c0 + 16 * h + e].dst[n] = y[e] + __uint_as_float(v[e]);
+            }
+            for (; anew != 0u; anew &= anew - 1) {
+                const int e = c0 + 16 * h + __ffs(anew) - 1;
+                if (e >= tile.count || n >= n1) continue;
+                const uint16_t *u = P.u + static_cast<int64_t>(tile.first + e) * P.u_cols + t.u_off;
+                const float s = plain_sum(B + n * t.sb_row, u, static_cast<int64_t>(P.ncols) * P.u_cols, r);
+                col[e].dst[n] = (col[e].base != nullptr ? col[e].base[n] : 0.0f) + s;
+            }
             if (h == 0) ask(c0 + 16);
         }
     }

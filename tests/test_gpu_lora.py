@@ -377,3 +377,88 @@ def test_lora_workspace_of_another_device_is_refused(q4k):
         q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], ws=q4k.Workspace(1 << 20, device="cpu"))
     got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], ranks=d["ranks"], scales=d["scales"], ws=q4k.Workspace(0, device="cuda"))
     check_exact(got, reference(d, use_base=False))
+
+
+@pytest.mark.parametrize("where", ["x", "A", "B", "all", "nan", "base"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(8, 300, 70, 2, 24), (64, 130, 33, 3, 72), (65, 300, 140, 2, 24), (300, 257, 300, 3, 72), (200, 640, 130, 2, 130)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_lora_infinite_values_follow_the_definition(q4k, shape, dtype, where):
+    """Infinities in x, A, B and base give the infinities (and inf - inf, 0 * inf: the NaN) of the definition, whatever
+    the number of columns, and every other value is exact."""
+    import torch
+    ncols, K, N, slots, rank = shape
+    d = make(sum(shape), *shape, dtype, ids="runs", ragged=False)
+    g = torch.Generator().manual_seed(1)
+
+    def put(t, n, value):
+        flat = t.view(-1)
+        at = torch.randperm(flat.numel(), generator=g)[:n].to(t.device)
+        flat[at] = (torch.randint(0, 2, (n,), generator=g) * 2 - 1).to(t.device, t.dtype) * value
+    d["A"][d["A"] == 0] = 0.5  # few products 0 * inf, so that most of what is hit is infinite
+    d["B"][:, ::2][d["B"][:, ::2] == 0] = -0.5
+    inf = float("inf")
+    if where in ("x", "all"):
+        put(d["x"], max(1, ncols // 8), inf)
+    if where in ("A", "all"):
+        put(d["A"], 2, inf)
+    if where in ("B", "all"):
+        put(d["B"], 5, inf)
+    if where == "nan":
+        put(d["x"], 2, float("nan"))
+        put(d["B"], 2, float("nan"))
+    if where == "base":
+        put(d["base"], 20, inf)
+    # term by term: a library's products may skip what they hold for zero
+    x, A, B = d["x"].double(), d["A"].double(), d["B"].double()
+    want = d["base"].double().clone()
+    for j, a in enumerate(d["ids"].tolist()):
+        if 0 <= a < slots:
+            want[j] += float(d["scales"][a]) * (B[a] * (A[a] * x[j]).sum(1)).sum(1)
+    got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], base=d["base"], ranks=d["ranks"], scales=d["scales"])
+    bad = ~((got.double() == want) | (got.isnan() & want.isnan()))
+    assert not bad.any(), f"{bad.sum()} of {bad.numel()}, first {bad.nonzero()[0].tolist()}: {got[bad][0]} for {want[bad][0]}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lora_largest_values_of_many_columns(q4k, dtype):
+    """The largest fp32 activations, and sums that overflow, in place over the base."""
+    import torch
+    big = torch.finfo(torch.float32).max
+    ncols, K, N, r = 130, 96, 200, 16
+    t = getattr(torch, dtype)
+    x = torch.zeros(ncols, K, device="cuda")
+    x[:, 5] = big
+    x[1::2, 7] = big
+    A, B = torch.zeros(1, r, K, device="cuda", dtype=t), torch.zeros(1, N, r, device="cuda", dtype=t)
+    A[0, 3, 5] = A[0, 3, 7] = 1.0
+    B[0, :, 3] = torch.where(torch.arange(N) % 3 == 0, -1.0, 1.0).to(t)
+    B[0, 1::2, 4] = 2.0  # meets a u of 0
+    y = torch.ones(ncols, N, device="cuda")
+    q4k.lora_add(x, A, B, torch.zeros(ncols, dtype=torch.int32, device="cuda"), base=y, out=y)
+    u = torch.where(torch.arange(ncols, device="cuda") % 2 == 1, float("inf"), big)
+    want = u[:, None] * B[0, :, 3].float()[None] + 1.0
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ncols", [8, 64, 65, 300])
+def test_lora_infinite_activations_with_positive_adapters(q4k, ncols, dtype):
+    """No terms of two signs: an infinite x, A or B makes its sums infinite and none NaN."""
+    import torch
+    d = make(ncols, ncols, 200, 140, 2, 40, dtype, ids="runs", ragged=False)
+    for k in ("A", "B"):
+        d[k] = d[k].abs() + 0.5
+    d["x"] = d["x"].abs() + 0.5
+    hit = torch.zeros(ncols, dtype=torch.bool, device="cuda")
+    hit[::3] = True
+    d["x"][hit, 77] = float("inf")
+    run = lambda: q4k.lora_add(d["x"], d["A"], d["B"], d["ids"], ranks=d["ranks"], scales=d["scales"])  # noqa: E731
+    got = run()
+    assert (got[hit] == float("inf")).all() and torch.isfinite(got[~hit]).all()
+    d["A"][0, 3, 5] = d["B"][1, 7, 9] = float("inf")
+    got = run()
+    assert (got[hit | (d["ids"] == 0)] == float("inf")).all()
+    rest = ~hit & (d["ids"] == 1)
+    assert (got[rest][:, 7] == float("inf")).all()
+    assert torch.isfinite(got[rest][:, torch.arange(140) != 7]).all()
