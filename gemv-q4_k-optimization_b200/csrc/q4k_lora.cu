@@ -363,7 +363,11 @@ cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream
 // products of pieces down to 2^-16 of the largest are summed on bf16 MMAs
 // (3 for bf16 weights, 5 for fp16, 6 for fp32); what is left out is below an
 // fp32 rounding. The MMAs' own sums are cut off, not rounded, so they are
-// taken over into fp32 registers after at most 12 of them.
+// taken over into fp32 sums: by the shrink after at most 12 of them, by the
+// expand after a chunk of 64 ranks (at most 24, the small products first).
+// Terms of one sign, in units of 2^-24: 1.5 off at any rank for bf16 weights, 3
+// for fp32; over the whole rank in one go it was 15 to 36 at rank 128, 88 to
+// 213 at 512, and 1 to 3 % faster there.
 constexpr int kTileCols = 64;  // columns per tile
 constexpr int kRanks = 64;     // ranks per shrink CTA
 constexpr int kStageK = 64;    // values of K per stage of A in shared memory
@@ -711,7 +715,7 @@ constexpr int kRows = 128;                     // rows of a tile
 constexpr int kChunkK = 64;                    // ranks of a chunk: one swizzled row of bf16
 constexpr int kUBytes = kTileCols * 128;       // one piece of u's chunk
 constexpr int kBBytes = kRows * 128;           // one piece of B's chunk
-constexpr int kTmemCols = 64;
+constexpr int kTmemCols = 64;                  // D; as many again for sums over several chunks
 template <typename T> constexpr size_t kExpandSmem = 3 * kUBytes + Weight<T>::kPieces * kBBytes + 1024;  // (+ alignment)
 
 __device__ __forceinline__ uint32_t swizzled(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
@@ -736,6 +740,22 @@ __device__ __forceinline__ void load_tmem(uint32_t (&v)[16], uint32_t addr) {
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
           "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr)
+        : "memory");
+}
+// Sums kept beside D, eight columns of this warp's 32 lanes at a time.
+__device__ __forceinline__ void load_tmem8(float (&v)[8], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void store_tmem8(uint32_t addr, const float (&v)[8]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+        "tcgen05.wait::st.sync.aligned;" ::"r"(addr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
         : "memory");
 }
 // Waits for a phase of the barrier, at most two seconds.
@@ -782,8 +802,9 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
         col[tid] = {t.base != nullptr ? t.base + j * t.sbase : nullptr, t.dst + j * t.sdst};
     }
     __syncwarp();
+    const int tmem_cols = r > kChunkK ? 2 * kTmemCols : kTmemCols;
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem)), "r"(kTmemCols)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem)), "r"(tmem_cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         if (lane == 0) {
@@ -833,7 +854,7 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem;
         if (tid == 0) {
-            bool add = c > 0;
+            bool add = false;
 #pragma unroll
             for (int order = 2; order >= 0; --order)  // small products first
 #pragma unroll
@@ -848,7 +869,7 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
             asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(&done))
                          : "memory");
         }
-        const bool last = c + 1 == chunks;
+        const bool last = c + 1 == chunks, first = c == 0;
         const int n = n0 + i * kRows + (warp & 3) * 32 + lane, c0 = warp / 4 * 32;
         float y[16];
         auto ask = [&](int from) {
@@ -868,12 +889,29 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
             if (chunks > 1) fill_u(c);
             fill_b(i, c);
         }
-        if (!last || bad) continue;
+        if (bad) continue;
+        uint32_t mine = d + ((warp & 3) * 32 << 16) + c0;
+        if (chunks > 1) {  // the chunk's sums are taken over into the kept ones
+            __syncwarp();
+#pragma unroll 1
+            for (int k = 0; k < 32; k += 8) {
+                float v[8], kept[8];
+                load_tmem8(v, mine + k);
+                if (!first) {
+                    load_tmem8(kept, mine + kTmemCols + k);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += kept[e];
+                }
+                store_tmem8(mine + kTmemCols + k, v);
+            }
+            if (!last) continue;
+            mine += kTmemCols;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t v[16];
             __syncwarp();
-            load_tmem(v, d + ((warp & 3) * 32 << 16) + c0 + 16 * h);
+            load_tmem(v, mine + 16 * h);
             float probe = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) probe = fmaf(__uint_as_float(v[e]), 0.0f, probe);
@@ -907,7 +945,7 @@ __global__ void __launch_bounds__(256, 4) k_lora_expand(const __grid_constant__ 
     __syncthreads();
     if (warp == 0) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
     }
 }
 

@@ -462,3 +462,21 @@ def test_lora_infinite_activations_with_positive_adapters(q4k, ncols, dtype):
     rest = ~hit & (d["ids"] == 1)
     assert (got[rest][:, 7] == float("inf")).all()
     assert torch.isfinite(got[rest][:, torch.arange(140) != 7]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 8, 256, 1, 64), (300, 8, 256, 1, 128), (70, 100, 33, 1, 200), (300, 8, 384, 1, 512),
+                                   (200, 1024, 512, 2, 512), (64, 8, 256, 1, 512)], ids=lambda s: "x".join(map(str, s)))
+def test_lora_accuracy_of_terms_of_one_sign(q4k, shape, dtype):
+    """Positive x, A and B: sums that are cut off instead of rounded would all err to one side, the more the larger the
+    rank. The bound is that of the file's head: sqrt(n) * 2^-24 of the 2-norm, n = K + rank + 1."""
+    import torch
+    ncols, K, N, slots, rank = shape
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    t = getattr(torch, dtype)
+    x, A, B = (torch.rand(s, device="cuda", generator=g) + 0.5 for s in ((ncols, K), (slots, rank, K), (slots, N, rank)))
+    d = dict(x=x, A=A.to(t), B=B.to(t), ids=torch.arange(ncols, dtype=torch.int32, device="cuda") % slots)
+    got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"])
+    want = reference(d, use_base=False)
+    err = torch.linalg.norm(got.double() - want).item() / torch.linalg.norm(want).item()
+    assert err <= (K + rank + 1) ** 0.5 * 2.0 ** -24, err * 2.0 ** 24
