@@ -362,12 +362,14 @@ cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream
 // that add up to it exactly (8 bits each), an fp16 weight into two, and the
 // products of pieces down to 2^-16 of the largest are summed on bf16 MMAs
 // (3 for bf16 weights, 5 for fp16, 6 for fp32); what is left out is below an
-// fp32 rounding. The MMAs' own sums are cut off, not rounded, so they are
-// taken over into fp32 sums: by the shrink after at most 12 of them, by the
+// fp32 rounding: two products of a second and a third piece, 2^-8 x 2^-17
+// each, of either sign. The MMAs' own sums are cut off, not rounded, so they
+// are taken over into fp32 sums: by the shrink after at most 12 of them, by the
 // expand after a chunk of 64 ranks (at most 24, the small products first).
-// Terms of one sign, in units of 2^-24: 1.5 off at any rank for bf16 weights, 3
-// for fp32; over the whole rank in one go it was 15 to 36 at rank 128, 88 to
-// 213 at 512, and 1 to 3 % faster there.
+// Terms of one sign come out 1.5 x 2^-24 off at any rank and type (3 for fp32
+// weights while pieces were cut off; the rounding costs no time); one sum over
+// the whole rank was 15 off at rank 128 and 88 at 512 (bf16 weights), and 1 to
+// 3 % faster there.
 constexpr int kTileCols = 64;  // columns per tile
 constexpr int kRanks = 64;     // ranks per shrink CTA
 constexpr int kStageK = 64;    // values of K per stage of A in shared memory
@@ -378,21 +380,19 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The upper halves of two fp32 values, a's in the lower half: bf16 pieces cut off towards zero.
-__device__ __forceinline__ uint32_t upper(float a, float b) {
-    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-}
-__device__ __forceinline__ float rest(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+// Two fp32 values as sums of bf16 pieces, a's in the lower half: each piece rounded to nearest, so that what is left
+// of it is at most 2^-8 of the value before (three pieces hold all 24 bits, two an fp16's 11) and of either sign.
 template <int N> __device__ __forceinline__ void pieces(float a, float b, uint32_t (&p)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        p[i] = upper(a, b);
-        a = rest(a);
-        b = rest(b);
+        const __nv_bfloat162 near = __floats2bfloat162_rn(a, b);
+        p[i] = *reinterpret_cast<const uint32_t *>(&near);
+        a -= __uint_as_float(p[i] << 16);
+        b -= __uint_as_float(p[i] & 0xffff0000u);
     }
 }
-// An infinity cut into pieces becomes inf, NaN, NaN, and times another's zero piece NaN. So what the MMAs give as
-// infinite or NaN is summed anew from the values themselves: it comes out as the fp32 sum, as with few columns.
+// An infinity cut into pieces becomes inf, NaN, NaN, and times another's zero piece NaN; values of kTop on round to
+// an infinite piece. So what the MMAs give as infinite or NaN is summed anew from the values themselves: it comes out as the fp32 sum, as with few columns.
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 template <typename T> __device__ __noinline__ float plain_dot(const T *a, const float *x, int K) {
     float s = 0.0f;
@@ -405,11 +405,15 @@ template <typename T> __device__ __noinline__ float plain_sum(const T *b, const 
     for (int k = 0; k < r; ++k) s = fmaf(to_f32(b[k]), value(k) + (value(piece + k) + value(2 * piece + k)), s);
     return s;
 }
-// Pieces that add up to any value: the first holds what is not finite.
+// Pieces that add up to any value: the first holds what is not finite, and of values of kTop on the upper half.
+constexpr float kTop = 0x1.ffp127f;
 __device__ __noinline__ void whole_pieces(float a, float b, uint32_t (&p)[3]) {
-    pieces(finite(a) ? a : 0.0f, finite(b) ? b : 0.0f, p);
-    if (!finite(a)) p[0] = (p[0] & 0xffff0000u) | (a != a ? 0x7fffu : __float_as_uint(a) >> 16);
-    if (!finite(b)) p[0] = (p[0] & 0xffffu) | (b != b ? 0x7fff0000u : __float_as_uint(b));
+    auto rest = [](float v) { return fabsf(v) < kTop ? v : finite(v) ? v - __uint_as_float(__float_as_uint(v) & 0xffff0000u) : 0.0f; };
+    auto first = [](float v) { return v != v ? 0x7fff0000u : __float_as_uint(v) & 0xffff0000u; };
+    pieces(rest(a), rest(b), p);
+    const bool ta = !(fabsf(a) < kTop), tb = !(fabsf(b) < kTop);
+    if (ta) p[2] = (p[2] & 0xffff0000u) | (p[1] & 0xffffu), p[1] = (p[1] & 0xffff0000u) | (p[0] & 0xffffu), p[0] = (p[0] & 0xffff0000u) | first(a) >> 16;
+    if (tb) p[2] = (p[2] & 0xffffu) | (p[1] & 0xffff0000u), p[1] = (p[1] & 0xffffu) | (p[0] & 0xffff0000u), p[0] = (p[0] & 0xffffu) | first(b);
 }
 template <typename T> struct Weight;  // bf16 pieces of a weight
 template <> struct Weight<__nv_bfloat16> { static constexpr int kPieces = 1; };
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
         const bool one = 2 * k < nr, two = 2 * k + 1 < nr;
         float2 w = make_float2(one ? v.x * scale : 0.0f, two ? v.y * scale : 0.0f);
         uint32_t p[3];
-        if (fmaf(w.x, 0.0f, w.y * 0.0f) == 0.0f) {
+        if (fabsf(w.x) < kTop && fabsf(w.y) < kTop) {
             pieces(w.x, w.y, p);
         } else {
             if (one && !finite(v.x)) w.x = plain_dot(A + 2 * k * t.sa_row, xcol[col], t.K) * scale;

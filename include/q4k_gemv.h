@@ -392,7 +392,11 @@ Q4K_API size_t q4k_noalloc_scratch_bytes(void);
 /* Low-rank adapters of many requests beside a shared projection:
  *   dst[j][n] = base[j][n] + scales[a] * sum_{t < ranks[a]} B[a][n][t] * (sum_k A[a][t][k] * x[j][k]),
  * a = ids[j], the adapter slot of column j; an id outside 0..slots-1 (by
- * convention -1) means no adapter: dst[j] = base[j].  All sums are fp32.
+ * convention -1) means no adapter: dst[j] = base[j].  All sums are fp32, of
+ * the values as they are whatever their type (up to 64 columns fused
+ * multiply-adds; more: tensor-core sums of at most 24 additions, which drop
+ * what lies below an fp32 sum's last place, added up in fp32).  Infinities and
+ * NaN come out as in these sums.
  * x, base and dst are fp32 columns as in q4k_task (base usually the GEMV's
  * dst).  A holds `slots` matrices of rank x K, B of nrows x rank; strides are
  * in elements, the innermost dimension is contiguous. */

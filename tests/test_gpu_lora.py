@@ -480,3 +480,22 @@ def test_lora_accuracy_of_terms_of_one_sign(q4k, shape, dtype):
     want = reference(d, use_base=False)
     err = torch.linalg.norm(got.double() - want).item() / torch.linalg.norm(want).item()
     assert err <= (K + rank + 1) ** 0.5 * 2.0 ** -24, err * 2.0 ** 24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lora_single_products_of_full_mantissas(q4k, dtype):
+    """K = rank = 1 and mantissas of ones behind the first eight bits, the worst for products of pieces. Per product,
+    in units of 2^-24 of it: what is left out (at most 2 * 2^-25 of a value's binade) 1, the last sum's cut-off (one step, 2^-23) 2,
+    the smaller sums' 2^-7 of that; the product with the scale (1) is exact. Two products: 6.1."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    t = getattr(torch, dtype)
+    ncols, N = 300, 500
+    x, A, B = (1 + 2.0**-7 - torch.randint(1, 9, s, device="cuda", generator=g) * 2.0**-23 for s in ((ncols, 1), (1, 1, 1), (1, N, 1)))
+    x[::2] += torch.rand(x[::2].shape, device="cuda", generator=g)
+    B[:, ::2] += torch.rand(B[:, ::2].shape, device="cuda", generator=g)
+    d = dict(x=x, A=A.to(t), B=B.to(t), ids=torch.zeros(ncols, dtype=torch.int32, device="cuda"))
+    want = reference(d, use_base=False)
+    got = q4k.lora_add(d["x"], d["A"], d["B"], d["ids"])
+    err = ((got.double() - want) / want).abs().max().item()
+    assert err <= 6.1 * 2.0 ** -24, err * 2.0 ** 24
