@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/Functions.h>
 
@@ -62,8 +63,8 @@ template <typename F> PyObject *guarded(F f) {
             Py_DECREF(e);
         }
     } catch (const PythonError &) {
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {  // torch's own, such as an allocation that does not fit
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

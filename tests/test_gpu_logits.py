@@ -309,3 +309,12 @@ def test_logits_largest_ids_in_lists_are_ignored(q4k, V, off):
     logits.copy_(t.pop("logits"))
     out = torch.empty_like(buf)[:, off:off + V]
     check(q4k.logits_process(logits, **t, out=out, pick=True), d)
+
+
+def test_an_output_that_does_not_fit_is_torchs_out_of_memory(q4k):
+    """A terabyte of new logits: the error that torch.empty raises, and the next call runs."""
+    import torch
+    row = torch.zeros(1, 1 << 18, device="cuda")
+    with pytest.raises(torch.OutOfMemoryError):
+        q4k.logits_process(row.expand(1 << 20, 1 << 18))
+    assert torch.equal(q4k.logits_process(row), row)
