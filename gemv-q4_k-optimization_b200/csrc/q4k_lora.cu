@@ -336,16 +336,26 @@ cudaError_t launch_cluster_of(const LoraParams &p, int ntasks, int rank, cudaStr
 
 template <typename T, int VA, int VB>
 cudaError_t launch_cluster(const LoraParams &p, int ntasks, int rank, cudaStream_t s) {
-    // One CTA fits on an SM, so 9 clusters of 16, 18 of 8 or 37 of 4 run at once. As long as a cluster for every column
-    // and task fits, sharing an adapter's bytes (they are in L2) gains less than the columns' arithmetic on one cluster
-    // costs; beyond that the clusters shrink, and then columns share. Measured at rank 32, bf16, K = 4096, us:
-    // 8 columns of one adapter, 1024 rows: one group of 8 11.2, a cluster for each 6.0;
-    // 12 columns of 16 adapters, 4096 rows: clusters of 16 10.9, of 8 6.7;
-    // 24 columns, 14336 rows, clusters of 8 in groups of 2: one adapter 13.0, 16 adapters 22.8; clusters of 4: 16.3 both;
+    // One CTA fits on an SM; by the times of calls of one cluster more, 7 clusters of 16, 15 of 8 or 33 of 4 run at once.
+    // As long as a cluster for every column and task fits, sharing an adapter's bytes (they are in L2) gains less than the
+    // columns' arithmetic on one cluster costs; beyond that the clusters shrink, and then columns share. Which columns
+    // have one adapter is not known here. Measured in a graph, us:
+    // 8 and 9 columns: clusters of 16 against 8: 4096 x 4096 rank 16 bf16 8.5 / 5.3, 1024 rows rank 8 7.9 / 4.7, 14336 rows
+    // rank 32 13.4 / 10.8; K = 14336 in fp32, 2.4 MB of weights each: 14.8 / 13.8 and 15.8 / 16.0, and 8.7 / 13.6 where
+    // one of 8 columns has no adapter, so these keep 16.
+    // 16 and 18 columns: clusters of 8 against 4: 9.7 / 7.2, rank 64 18.6 / 15.2, 14336 rows 20.2 / 17.0, 14336 in fp32 34.9 / 33.2.
+    // 24 (8 columns of q, k, v, rank 64 fp16): clusters of 4 15.2 with one adapter, 16.3 with eight; of 8 in groups of 2
+    // 10.7 and 18.2.
+    // 36 (12 columns of q, k, v): clusters of 4 19.4 with one adapter, 23.6 with twelve; in groups of 2 16.6 and 25.5.
     // 48 columns of 16 adapters, 4096 rows: clusters of 8 in groups of 4 14.5, of 4 in groups of 2 10.9.
+    // 56 (8 columns of 7 projections, rank 16, eight adapters): clusters of 4 in groups of 4 18.3, one by one 13.5; 64 columns
+    // of 16 adapters at random, 14336 rows: in groups of 4 24.8, of 2 31.5.
     const int pieces = p.ncols * ntasks;
-    return pieces <= 9    ? launch_cluster_of<T, VA, VB, 1, 16>(p, ntasks, rank, s)
-           : pieces <= 18 ? launch_cluster_of<T, VA, VB, 1, 8>(p, ntasks, rank, s)
+    int64_t bytes = 0;  // of weights per piece
+    for (int i = 0; i < ntasks; ++i)
+        bytes = std::max<int64_t>(bytes, (p.task[i].K + static_cast<int64_t>(p.task[i].nrows)) * p.task[i].rank * sizeof(T));
+    return pieces <= 7 || (pieces <= 9 && bytes >= 2000000) ? launch_cluster_of<T, VA, VB, 1, 16>(p, ntasks, rank, s)
+           : pieces <= 15 ? launch_cluster_of<T, VA, VB, 1, 8>(p, ntasks, rank, s)
            : pieces <= 37 ? launch_cluster_of<T, VA, VB, 1, 4>(p, ntasks, rank, s)
            : pieces <= 48 ? launch_cluster_of<T, VA, VB, 2, 4>(p, ntasks, rank, s)
                           : launch_cluster_of<T, VA, VB, 4, 4>(p, ntasks, rank, s);
