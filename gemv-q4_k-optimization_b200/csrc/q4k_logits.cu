@@ -463,7 +463,8 @@ cudaError_t launch_logits(const LogitsParams &p, int ncols, cudaStream_t s) {
     int nc = 1;
     while (nc < 16 && nc * kChunk < p.nvocab && nc * static_cast<int64_t>(ncols) < 1184) nc *= 2;
     // slots for a column's whole history and its likely biases (their number per column is known to the device
-    // alone); a CTA whose tokens need more takes them in smaller segments
+    // alone); a CTA whose tokens need more takes them in smaller segments, its whole slice from then on, and reads the
+    // column's lists again for each: right, but slow for a column that holds most of a batch's biases
     const int64_t listed = p.max_history + (p.bias_tokens != nullptr ? 2 * static_cast<int64_t>(p.n_bias) / ncols + 64 : 0);
     LogitsParams q = p;
     q.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, std::max<int64_t>(kMinSlots, (listed + 31) / 32 * 32)));
