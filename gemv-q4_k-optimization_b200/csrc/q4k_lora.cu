@@ -406,24 +406,30 @@ template <int N> __device__ __forceinline__ void pieces(float a, float b, uint32
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 template <typename T> __device__ __noinline__ float plain_dot(const T *a, const float *x, int K) {
     float s = 0.0f;
-    for (int k = 0; k < K; ++k) s = fmaf(to_f32(a[k]), x[k], s);
+    for (int k = 0; k < K && s == s; k += 8)  // (NaN stays: columns of NaN end at once)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (k + e < K) s = fmaf(to_f32(a[k + e]), x[k + e], s);
     return s;
 }
 template <typename T> __device__ __noinline__ float plain_sum(const T *b, const uint16_t *u, int64_t piece, int r) {
     auto value = [&](int64_t i) { return __uint_as_float(static_cast<uint32_t>(u[i]) << 16); };
     float s = 0.0f;
-    for (int k = 0; k < r; ++k) s = fmaf(to_f32(b[k]), value(k) + (value(piece + k) + value(2 * piece + k)), s);
+#pragma unroll 1
+    for (int k = 0; k < r && s == s; ++k) s = fmaf(to_f32(b[k]), value(k) + (value(piece + k) + value(2 * piece + k)), s);
     return s;
 }
 // Pieces that add up to any value: the first holds what is not finite, and of values of kTop on the upper half.
 constexpr float kTop = 0x1.ffp127f;
-__device__ __noinline__ void whole_pieces(float a, float b, uint32_t (&p)[3]) {
+__device__ __noinline__ uint3 whole_pieces(float a, float b) {
     auto rest = [](float v) { return fabsf(v) < kTop ? v : finite(v) ? v - __uint_as_float(__float_as_uint(v) & 0xffff0000u) : 0.0f; };
     auto first = [](float v) { return v != v ? 0x7fff0000u : __float_as_uint(v) & 0xffff0000u; };
+    uint32_t p[3];
     pieces(rest(a), rest(b), p);
     const bool ta = !(fabsf(a) < kTop), tb = !(fabsf(b) < kTop);
     if (ta) p[2] = (p[2] & 0xffff0000u) | (p[1] & 0xffffu), p[1] = (p[1] & 0xffff0000u) | (p[0] & 0xffffu), p[0] = (p[0] & 0xffff0000u) | first(a) >> 16;
     if (tb) p[2] = (p[2] & 0xffffu) | (p[1] & 0xffff0000u), p[1] = (p[1] & 0xffffu) | (p[0] & 0xffff0000u), p[0] = (p[0] & 0xffffu) | first(b);
+    return make_uint3(p[0], p[1], p[2]);
 }
 template <typename T> struct Weight;  // bf16 pieces of a weight
 template <> struct Weight<__nv_bfloat16> { static constexpr int kPieces = 1; };
@@ -707,7 +713,8 @@ __global__ void __launch_bounds__(256, 2) k_lora_shrink(const __grid_constant__ 
         } else {
             if (one && !finite(v.x)) w.x = plain_dot(A + 2 * k * t.sa_row, xcol[col], t.K) * scale;
             if (two && !finite(v.y)) w.y = plain_dot(A + (2 * k + 1) * t.sa_row, xcol[col], t.K) * scale;
-            whole_pieces(w.x, w.y, p);
+            const uint3 q3 = whole_pieces(w.x, w.y);
+            p[0] = q3.x, p[1] = q3.y, p[2] = q3.z;
         }
 #pragma unroll
         for (int e = 0; e < 3; ++e)
