@@ -312,11 +312,12 @@ Q4K_API int q4k_gather_wait(const q4k_gather *gather, void *workspace, size_t wo
  * words in a known state on entry: zero the workspace once with
  * q4k_workspace_init before the first call; every call that completes leaves
  * them valid again (the other calls may use the same workspace in between,
- * in launches of up to 524288 rows; a larger one needs q4k_workspace_init
- * before the next single-launch call).  After a call reports Q4K_ETIMEOUT (q4k_workspace_status) call
- * q4k_workspace_init again.  gather may be NULL (no all-gather) or a
- * descriptor as for q4k_gemv_batch_allgather; the launch then waits for the
- * previous gathering call's rows before it reads its activations. */
+ * where the single-launch calls have up to 524288 rows, each task's rounded up
+ * to 32; larger ones need q4k_workspace_init again behind other calls).  After
+ * a call reports Q4K_ETIMEOUT (q4k_workspace_status) call q4k_workspace_init
+ * again.  gather may be NULL (no all-gather) or a descriptor as for
+ * q4k_gemv_batch_allgather; the launch then waits for the previous gathering
+ * call's rows before it reads its activations. */
 Q4K_API int q4k_workspace_init(void *workspace, size_t workspace_bytes, q4k_stream_t stream);
 Q4K_API int q4k_gemv_batch_persistent(const q4k_task *tasks, int ntasks, int ncols, const q4k_gather *gather,
                                       void *workspace, size_t workspace_bytes, q4k_stream_t stream);
@@ -428,9 +429,9 @@ typedef struct q4k_lora_task {
  * tasks (at most Q4K_MAX_TASKS).  Up to 64 columns take one launch and no
  * workspace (q4k_lora_workspace_bytes 0); more take three launches, whose
  * workspace need not be initialised (a wait that gives up after 2 s leaves
- * Q4K_ETIMEOUT in its status word, see q4k_workspace_status).  Of a workspace
- * shared with the GEMV calls only that word of the control words changes, so
- * q4k_gemv_batch_persistent needs no new q4k_workspace_init behind it. */
+ * Q4K_ETIMEOUT in its status word, see q4k_workspace_status); a workspace
+ * shared with q4k_gemv_batch_persistent stays valid for it as with the other
+ * calls. */
 Q4K_API size_t q4k_lora_workspace_bytes(const q4k_lora_task *tasks, int ntasks, int ncols);
 Q4K_API int q4k_lora_batch(const q4k_lora_task *tasks, int ntasks, int ncols, const int32_t *ids, void *workspace,
                            size_t workspace_bytes, q4k_stream_t stream);
